@@ -676,6 +676,7 @@ void bind_gdn(pybind11::module_& m);
 void bind_comm(pybind11::module_& m);
 void bind_quant(pybind11::module_& m);
 void bind_ep(pybind11::module_& m);
+void bind_kv8(pybind11::module_& m);
 void bind_layers(pybind11::module_& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -750,6 +751,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_comm(m);
   bind_quant(m);
   bind_ep(m);
+  bind_kv8(m);
 #endif
   bind_layers(m);
 }

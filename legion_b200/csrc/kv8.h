@@ -1,0 +1,48 @@
+// Launch interface of the 8-bit key/value cache (kv8_cache.cu, attn_kv8_decode_sm100.cu). A cache is e4m3 codes
+// [blocks, kv heads, page, head size] for keys and for values and one float32 scale, a power of two, per block and head
+// [blocks, kv heads]; a value is its code times its block's scale. Pointers are device pointers; every function returns 0 on
+// success and enqueues without synchronising.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace lb {
+
+struct Kv8Cache {
+  uint8_t* k; uint8_t* v;
+  float* k_scale; float* v_scale;
+  int n_blocks, Hkv, page, dk, dv;
+};
+
+// Sequences of a call: sequence i owns query (or new) rows cu[i] .. cu[i + 1], the last of its ctx[i] tokens, which lie in the
+// blocks of row i of the table.
+struct Kv8Seqs {
+  const int* table; long ld_table; int width;
+  const int* ctx; const int* cu;
+  int n, max_new;
+  long T;                          // rows of the call
+  int* status;
+};
+
+struct Kv8Append {
+  const void* k; long k_tok, k_head;    // bf16 [T, kv heads, dk]: elements between tokens and between heads
+  const void* v; long v_tok, v_head;
+};
+int kv8_append_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Append& a, cudaStream_t st);
+
+struct Kv8Attn {
+  const void* q; long q_tok, q_head;    // bf16 [T, Hq, dk]
+  int Hq;
+  float scale, softcap;
+  int window;
+  const float* sink;                    // [Hq] or nullptr
+  void* out; long o_tok;                // bf16 [T, Hq * dv], elements between rows
+  float* lse;                           // [T, Hq] log2 of the sum of the exponentials, or nullptr
+};
+// Decode (max_new == 1): tiles of 128 keys, `per` of them to a split. part: splits of every row and head, dv + 2 floats each
+// (splits = ceil(ceil(max_ctx / 128) / per), 1 needs none).
+int kv8_decode_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int per, int n_splits, float* part, cudaStream_t st);
+const char* kv8_last_error();
+void kv8_set_error(const char* what);
+
+}  // namespace lb

@@ -11,6 +11,7 @@ import torch
 
 from . import reference as _ref
 from . import sm100 as _sm
+from .kv8 import Kv8Cache, kv8_append, kv8_attention
 
 reference = _ref
 sm100 = _sm

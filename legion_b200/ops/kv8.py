@@ -1,0 +1,106 @@
+"""The 8-bit key/value cache: paged e4m3 codes with one scale per block of tokens and head, and the operators on it.
+
+A value is its code times the scale of its block and head. Scales are powers of two, 2^(e - 7) for a block whose largest magnitude
+lies in [2^e, 2^(e+1)) and at least 2^-60 (0: nothing but zeros). e4m3 is a floating format, so a power of two costs no precision,
+a block whose scale grows keeps its older codes bit for bit down to its smallest normal value, and codes move between blocks
+exactly. NaN is stored as NaN; infinities count as the largest finite bf16 value.
+
+Sequences are given as everywhere in ``ops``: ``block_table`` int32 [sequences, blocks], ``ctx_lens`` int32 the tokens a sequence
+holds with the call's rows, ``cu_q`` int32 [sequences + 1] bounds of its rows, which are the last of its tokens. On CUDA every
+call enqueues on the current stream, takes its scratch from the allocator (calls on other streams and captured graphs share none)
+and checks shapes, types and devices; what is wrong with them raises ValueError. Table entries outside the cache are not followed:
+the kernels record them in the workspace's status word. CPU tensors run the float32 forms of ``ops.reference``.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import reference as _ref
+from . import sm100 as _sm
+
+
+class Kv8Cache:
+    """``k`` float8_e4m3fn [blocks, kv heads, page, head size], ``v`` likewise with its own head size, ``k_scale`` and ``v_scale``
+    float32 [blocks, kv heads], powers of two or 0."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+
+    @classmethod
+    def empty(cls, n_blocks: int, page: int, kv_heads: int, dk: int, dv: Optional[int] = None, device="cpu") -> "Kv8Cache":
+        def codes(d):
+            return torch.zeros(n_blocks, kv_heads, page, d, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+        s = torch.zeros(2, n_blocks, kv_heads, device=device)
+        return cls(codes(dk), codes(dv or dk), s[0], s[1])
+
+    @property
+    def page(self) -> int:
+        return self.k.shape[2]
+
+    def bytes_per_block(self) -> int:
+        return self.k[0].numel() + self.v[0].numel() + 8 * self.k.shape[1]
+
+
+def _check(cache: Kv8Cache, who: str):
+    k, v = cache.k, cache.v
+    if k.dim() != 4 or v.dim() != 4 or k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or k.shape[:3] != v.shape[:3]:
+        raise ValueError(f"{who}: codes are float8_e4m3fn [blocks, kv heads, page, head size]")
+    for s in (cache.k_scale, cache.v_scale):
+        if s.dtype != torch.float32 or s.shape != k.shape[:2]:
+            raise ValueError(f"{who}: scales are float32 [blocks, kv heads]")
+
+
+def kv8_append(cache: Kv8Cache, k, v, block_table, ctx_lens, cu_q, max_q_len: int) -> None:
+    """Writes the rows' keys and values (``k`` [T, kv heads, dk], ``v`` [T, kv heads, dv], rows and heads may lie apart) to the
+    cache. A block that gets its first cell begins anew: its other cells become zero. In others the scale grows where a new value
+    needs it, and the older codes are rounded to it. A block that gets tokens belongs to one sequence of the call."""
+    if k.is_cuda:
+        _sm.ext().kv8_append(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, block_table, ctx_lens, cu_q, max_q_len,
+                             _sm.Workspace.get(k.device).status)
+        return
+    _check(cache, "kv8_append")
+    if k.dim() != 3 or v.dim() != 3 or k.shape[:2] != v.shape[:2] or k.shape[1:] != cache.k.shape[1::2] or v.shape[1:] != cache.v.shape[1::2]:
+        raise ValueError("kv8_append: rows [T, kv heads, head size] do not fit the cache")
+    _ref.kv8_append(cache, k, v, block_table, ctx_lens, cu_q)
+
+
+def _decode_split(n: int, kv_heads: int, group: int, tiles: int) -> Tuple[int, int]:
+    """(tiles of 128 keys to a split, splits) of a decode call."""
+    s = _sm.decode_splits(n, kv_heads, (group + 15) // 16, tiles * 128)
+    per = -(-tiles // s)
+    return per, -(-tiles // per)
+
+
+def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: int, scale: float, window: int = 0, softcap: float = 0.0,
+                  sink=None, weights=None, observe: int = 0, max_ctx: Optional[int] = None, out=None):
+    """Causal attention of the query rows ``q`` [T, heads, dk] over the cache; returns [T, heads, dv] (``out`` takes it; its rows
+    may lie apart). ``window`` > 0: the last that many keys are visible; ``softcap`` > 0: scores become softcap * tanh(score /
+    softcap); ``sink`` [heads] float32: exp(sink) joins the denominator. A row that sees no key is zero. ``max_q_len`` == 1 selects
+    the decode kernel. ``max_ctx``: bound of the lengths, for the split over the keys (None: the table's)."""
+    if weights is not None:
+        raise NotImplementedError("kv8_attention: sums of weights")
+    if not q.is_cuda:
+        _check(cache, "kv8_attention")
+        if q.dim() != 3 or q.shape[2] != cache.k.shape[3] or q.shape[1] % cache.k.shape[1]:
+            raise ValueError("kv8_attention: queries [T, heads, head size] do not fit the cache")
+        if window < 0 or softcap < 0:
+            raise ValueError("kv8_attention: window and soft cap are not negative")
+        o = _ref.kv8_attention(q, cache, block_table, ctx_lens, cu_q, scale, window, softcap, sink)
+        return o if out is None else out.copy_(o)
+    if max_q_len > 1:
+        raise NotImplementedError("kv8_attention: prompts")
+    k = cache.k
+    if out is None:
+        out = torch.empty(q.shape[0], q.shape[1], cache.v.shape[3], dtype=q.dtype, device=q.device)
+    span = min(max_ctx or 1 << 30, block_table.shape[1] * k.shape[2])
+    tiles = max(1, -(-span // 128))
+    if window > 0:
+        tiles = min(tiles, -(-window // 128) + 1)
+    per, splits = _decode_split(block_table.shape[0], k.shape[1], q.shape[1] // k.shape[1], tiles)
+    _sm.ext().kv8_attention(q, k, cache.v, cache.k_scale, cache.v_scale, block_table, ctx_lens, cu_q, max_q_len, scale, window,
+                            softcap, sink, per, splits, out, _sm.Workspace.get(q.device).status)
+    return out

@@ -650,3 +650,76 @@ def sample(logits, temperature, top_k, top_p, min_p, generator=None):
         p = torch.where(mask, p, torch.zeros_like(p))
     p = p / p.sum()
     return int(torch.multinomial(p, 1, generator=generator))
+
+
+# ------------------------------------------------------------------------------------------ 8-bit key/value cache
+def kv8_scale_of(amax):
+    """Block scale of a largest magnitude (``ops.kv8``)."""
+    e = torch.frexp(amax.float()).exponent - 1
+    power = (((e - 7).clamp_min(-60) + 127) << 23).view(torch.float32)
+    return torch.where(amax > 0, power, torch.zeros_like(power))
+
+
+def _kv8_values(codes, scale, blocks):
+    """Cached rows [tokens, kv heads, dim] of a list of blocks, float32."""
+    x = codes.view(torch.uint8)[blocks].view(codes.dtype).float() * scale[blocks][..., None, None]
+    return x.transpose(1, 2).flatten(0, 1)
+
+
+def kv8_append(cache, k, v, block_table, ctx_lens, cu_q):
+    page = cache.k.shape[2]
+    most = torch.finfo(torch.bfloat16).max
+    for x, codes, scale in ((k, cache.k, cache.k_scale), (v, cache.v, cache.v_scale)):
+        raw = codes.view(torch.uint8)
+        for i in range(len(ctx_lens)):
+            q0, q1, ctx = int(cu_q[i]), int(cu_q[i + 1]), int(ctx_lens[i])
+            at = ctx - (q1 - q0)
+            while at < ctx:
+                end = min(ctx, (at // page + 1) * page)
+                if end <= 0:
+                    at = end
+                    continue
+                at = max(at, 0)
+                blk, c0 = int(block_table[i, at // page]), at % page
+                rows = x[q1 - (ctx - at):q1 - (ctx - end)].float().clamp(-most, most).transpose(0, 1)
+                if c0 == 0:
+                    raw[blk], scale[blk] = 0, 0
+                now = torch.maximum(scale[blk], kv8_scale_of(rows.abs().nan_to_num(nan=0.0).amax((1, 2))))
+                inv = torch.where(now > 0, 1 / now, torch.zeros_like(now))[:, None, None]
+                grown = (raw[blk].view(codes.dtype).float() * (scale[blk][:, None, None] * inv)).to(codes.dtype).view(torch.uint8)
+                raw[blk] = torch.where(((now != scale[blk]) | (now == 0))[:, None, None], grown, raw[blk])
+                raw[blk, :, c0:c0 + end - at] = (rows * inv).clamp(-448, 448).to(codes.dtype).view(torch.uint8)
+                scale[blk] = now
+                at = end
+
+
+def kv8_attention(q, cache, block_table, ctx_lens, cu_q, scale, window: int = 0, softcap: float = 0.0, sink=None):
+    T, Hq, _ = q.shape
+    Hkv, page = cache.k.shape[1], cache.k.shape[2]
+    out = q.new_zeros(T, Hq, cache.v.shape[3])
+    for i in range(len(ctx_lens)):
+        q0, q1, ctx = int(cu_q[i]), int(cu_q[i + 1]), int(ctx_lens[i])
+        if q1 <= q0 or ctx <= 0:
+            continue
+        blocks = block_table[i, :-(-ctx // page)].long()
+        k = _kv8_values(cache.k, cache.k_scale, blocks)[:ctx].repeat_interleave(Hq // Hkv, dim=1)
+        v = _kv8_values(cache.v, cache.v_scale, blocks)[:ctx].repeat_interleave(Hq // Hkv, dim=1)
+        s = torch.einsum("qhd,khd->hqk", q[q0:q1].float(), k) * scale
+        if softcap > 0:
+            s = torch.tanh(s / softcap) * softcap
+        pos = torch.arange(ctx - (q1 - q0), ctx, device=q.device)[:, None]
+        key = torch.arange(ctx, device=q.device)
+        hidden = key > pos
+        if window > 0:
+            hidden = hidden | (key <= pos - window)
+        s = s.masked_fill(hidden, float("-inf"))
+        if sink is not None:
+            s = torch.cat([s, sink.float().view(Hq, 1, 1).expand(Hq, q1 - q0, 1)], dim=-1)
+        p = torch.softmax(s, dim=-1)[..., :ctx]
+        p = torch.where(hidden.all(1)[None, :, None], torch.zeros_like(p), p)
+        bad = v.isnan()                       # a NaN value reaches the rows that see it and no others
+        o = torch.einsum("hqk,khd->qhd", p, v.masked_fill(bad, 0.0))
+        if bool(bad.any()):
+            o = o.masked_fill(torch.einsum("qk,khd->qhd", (~hidden).float(), bad.float()) > 0, float("nan"))
+        out[q0:q1] = o.to(q.dtype)
+    return out
