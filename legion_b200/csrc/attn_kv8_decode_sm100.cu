@@ -534,17 +534,26 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   }
 }
 
-// Joins the splits of a row and head: sum over splits of 2^(m - M) O, over the sum of 2^(m - M) l (and a sink).
+// Joins the splits of a row and head: sum over splits of 2^(m - M) O, over the sum of 2^(m - M) l (and a sink). Splits of a decode
+// row that got no tiles left no partial results; those of prompt rows (ROWS: one CTA per row and head) all did.
+template <bool ROWS>
 __global__ void __launch_bounds__(128) kv8_combine_kernel(const DecodeArgs p) {
   __shared__ float s_w[129];
   griddep_wait();
   griddep_launch();
-  const int b = blockIdx.y, h = blockIdx.x, D = p.c.dv;
-  const int row = p.s.cu[b];
-  if (p.s.cu[b + 1] != row + 1 || row < 0 || row >= p.s.T) return;
-  const int ctx = int(min(long(max(p.s.ctx[b], 0)), long(p.s.width) * p.c.page));
-  const int start = (p.a.window > 0 && ctx > p.a.window) ? ctx - p.a.window : 0;
-  const int live = min(p.n_splits, ((ctx + 127) / 128 - start / 128 + p.per - 1) / p.per);
+  const int D = p.c.dv, h = blockIdx.x % p.a.Hq;
+  long row = blockIdx.x / p.a.Hq;
+  int live = p.n_splits;
+  if (!ROWS) {
+    const int b = int(row);
+    row = p.s.cu[b];
+    if (p.s.cu[b + 1] != row + 1 || row < 0 || row >= p.s.T) return;
+    const int ctx = int(min(long(max(p.s.ctx[b], 0)), long(p.s.width) * p.c.page));
+    const int start = (p.a.window > 0 && ctx > p.a.window) ? ctx - p.a.window : 0;
+    live = min(p.n_splits, ((ctx + 127) / 128 - start / 128 + p.per - 1) / p.per);
+  } else if (row < p.s.cu[0] || row >= p.s.cu[p.s.n]) {
+    return;                                                 // a row of no sequence
+  }
   const float* part = p.part + (long(row) * p.a.Hq + h) * p.n_splits * (D + 2);
   const float sk = p.a.sink ? p.a.sink[h] * 1.4426950408889634f : -INFINITY;
   if (threadIdx.x < 32) {
@@ -589,6 +598,12 @@ cudaError_t launch(const CUtensorMap* tk, const CUtensorMap* tv, const DecodeArg
 
 }  // namespace
 
+cudaError_t kv8_join(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int n_splits, float* part, cudaStream_t st) {
+  const DecodeArgs p{c, s, a, 0, n_splits, 0.f, 0.f, part};
+  kv8_combine_kernel<true><<<unsigned(s.T * a.Hq), 128, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
 int kv8_decode_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int per, int n_splits, float* part, cudaStream_t st) {
   if (s.n <= 0 || s.T <= 0) return 0;
   const uint64_t rows = uint64_t(c.n_blocks) * c.Hkv * c.page;
@@ -610,7 +625,7 @@ int kv8_decode_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int
   if (kh == K_ && mt == V_ && nq == Q_) e = cap ? launch<K_, V_, Q_, true>(tk, tv, p, st) : launch<K_, V_, Q_, false>(tk, tv, p, st);
   LB_KV8(1, 1, 8) LB_KV8(1, 1, 16) LB_KV8(2, 2, 8) LB_KV8(2, 2, 16) LB_KV8(1, 2, 8) LB_KV8(1, 2, 16) LB_KV8(2, 1, 8) LB_KV8(2, 1, 16)
 #undef LB_KV8
-  if (e == cudaSuccess && n_splits > 1) e = launch_pdl(kv8_combine_kernel, dim3(a.Hq, s.n), dim3(128), 0, st, p);
+  if (e == cudaSuccess && n_splits > 1) e = launch_pdl(kv8_combine_kernel<false>, dim3(unsigned(a.Hq) * s.n), dim3(128), 0, st, p);
   if (e != cudaSuccess) kv8_set_error(cudaGetErrorString(e));
   return e != cudaSuccess;
 }

@@ -92,11 +92,13 @@ void kv8_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   one_device(q, {&k, &v, &ks, &vs, &table, &ctx, &cu, &out, &status}, who);
   c10::cuda::CUDAGuard guard(q.device());
   if (T == 0 || s.n == 0 || max_new == 0) return;
-  LB_ASK(per >= 1 && n_splits >= 1 && n_splits <= 128, who, ": splits");
+  LB_ASK(per >= 1 && n_splits >= 1 && n_splits <= 128 && n_splits * c.Hkv <= 65535 && T * Hq < (int64_t(1) << 31), who, ": splits, rows");
   Tensor part;
   if (n_splits > 1) part = at::empty({T * Hq * n_splits * (c.dv + 2)}, q.options().dtype(at::kFloat));
-  TORCH_CHECK(lb::kv8_decode_launch(c, s, a, int(per), int(n_splits), n_splits > 1 ? part.data_ptr<float>() : nullptr, cur_stream()) == 0,
-              "kv8_attention: ", lb::kv8_last_error());
+  float* pp = n_splits > 1 ? part.data_ptr<float>() : nullptr;
+  const int rc = max_new == 1 ? lb::kv8_decode_launch(c, s, a, int(per), int(n_splits), pp, cur_stream())
+                              : lb::kv8_prompt_launch(c, s, a, int(n_splits), pp, cur_stream());
+  TORCH_CHECK(rc == 0, "kv8_attention: ", lb::kv8_last_error());
 }
 }  // namespace
 

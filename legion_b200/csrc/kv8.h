@@ -42,6 +42,10 @@ struct Kv8Attn {
 // Decode (max_new == 1): tiles of 128 keys, `per` of them to a split. part: splits of every row and head, dv + 2 floats each
 // (splits = ceil(ceil(max_ctx / 128) / per), 1 needs none).
 int kv8_decode_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int per, int n_splits, float* part, cudaStream_t st);
+// Prompts and rows behind a context: the tiles of 128 keys that a tile of rows sees fall into n_splits parts; part as above.
+int kv8_prompt_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int n_splits, float* part, cudaStream_t st);
+// Joins the partial results of every row and head of a prompt call.
+cudaError_t kv8_join(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int n_splits, float* part, cudaStream_t st);
 const char* kv8_last_error();
 void kv8_set_error(const char* what);
 

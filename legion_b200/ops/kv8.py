@@ -13,6 +13,7 @@ the kernels record them in the workspace's status word. CPU tensors run the floa
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -68,11 +69,25 @@ def kv8_append(cache: Kv8Cache, k, v, block_table, ctx_lens, cu_q, max_q_len: in
     _ref.kv8_append(cache, k, v, block_table, ctx_lens, cu_q)
 
 
+@functools.lru_cache(maxsize=4096)
 def _decode_split(n: int, kv_heads: int, group: int, tiles: int) -> Tuple[int, int]:
     """(tiles of 128 keys to a split, splits) of a decode call."""
     s = _sm.decode_splits(n, kv_heads, (group + 15) // 16, tiles * 128)
     per = -(-tiles // s)
     return per, -(-tiles // per)
+
+
+@functools.lru_cache(maxsize=4096)
+def _prompt_splits(n: int, kv_heads: int, rows: int, row_tile: int, tiles: int) -> int:
+    """Parts of a prompt call's keys: as many as make the waves of CTAs times their tiles (and what a part costs beside them)
+    least."""
+    ctas = n * kv_heads * -(-rows // row_tile)
+    best, cost = 1, None
+    for s in range(1, min(32, tiles) + 1):
+        c = -(-ctas * s // _sm.NUM_SMS) * (-(-tiles // s) + (4 if s == 1 else 7))
+        if cost is None or c < cost:
+            best, cost = s, c
+    return best
 
 
 def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: int, scale: float, window: int = 0, softcap: float = 0.0,
@@ -91,8 +106,6 @@ def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: in
             raise ValueError("kv8_attention: window and soft cap are not negative")
         o = _ref.kv8_attention(q, cache, block_table, ctx_lens, cu_q, scale, window, softcap, sink)
         return o if out is None else out.copy_(o)
-    if max_q_len > 1:
-        raise NotImplementedError("kv8_attention: prompts")
     k = cache.k
     if out is None:
         out = torch.empty(q.shape[0], q.shape[1], cache.v.shape[3], dtype=q.dtype, device=q.device)
@@ -100,7 +113,12 @@ def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: in
     tiles = max(1, -(-span // 128))
     if window > 0:
         tiles = min(tiles, -(-window // 128) + 1)
-    per, splits = _decode_split(block_table.shape[0], k.shape[1], q.shape[1] // k.shape[1], tiles)
+    group = q.shape[1] // k.shape[1]
+    if max_q_len == 1:
+        per, splits = _decode_split(block_table.shape[0], k.shape[1], group, tiles)
+    else:
+        rows = 256 if k.shape[3] <= 128 and cache.v.shape[3] <= 128 else 128
+        per, splits = 1, _prompt_splits(block_table.shape[0], k.shape[1], max_q_len * group, rows, tiles + max_q_len // 128)
     _sm.ext().kv8_attention(q, k, cache.v, cache.k_scale, cache.v_scale, block_table, ctx_lens, cu_q, max_q_len, scale, window,
                             softcap, sink, per, splits, out, _sm.Workspace.get(q.device).status)
     return out

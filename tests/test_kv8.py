@@ -3,7 +3,7 @@ reference ops, on a GPU the kernels.
 
 Tolerances of the attention, fixed beforehand: an output of bf16 is off by 2^-8 of itself (its rounding) and by the error of the
 probabilities times sum p |v|. A probability is off by 2^-9 (three e5m2 terms, or one half) and by the error of its score, twice
-(numerator and denominator): queries split into 8-bit terms keep 2^-21 of the largest query value, sums of D products in 32 bits
+(numerator and denominator): queries split into 8-bit terms keep 2^-21 of the largest query value (prompts: 2^-17 of the row's), sums of D products in 32 bits
 D 2^-23 of the sum of magnitudes, the soft cap 2^-19 of the cap. A key's weight, its probability times the scale of its values, is
 also off by up to 2^-30 of the largest weight of its row: e5m2 ends at a step of 2^-16, and the largest weight lies at 2^13 or above."""
 import math
@@ -148,7 +148,7 @@ def attend(q, cache, table, lens, new, scale, window=0, softcap=0.0, sink=None):
             qh = q[cu[i]:cu[i + 1], h].double().cpu()
             s = qh @ k.T * scale
             most = (qh.abs().nan_to_num(0, 0, 0) @ k.abs().nan_to_num().T * scale)
-            off = float(most.max()) * D * 2.0 ** -23 + 2.0 ** -21 * float(q[cu[i]:cu[i + 1]].abs().float().nan_to_num(0, 0, 0).max()) * float(k.abs().nan_to_num().sum(1).max()) * abs(scale)
+            off = float(most.max()) * D * 2.0 ** -23 + 2.0 ** (-21 if max(new) == 1 else -17) * float(q[cu[i]:cu[i + 1]].abs().float().nan_to_num(0, 0, 0).max()) * float(k.abs().nan_to_num().sum(1).max()) * abs(scale)
             if softcap:
                 s, off = softcap * torch.tanh(s / softcap), off + softcap * 2.0 ** -19
             s = s.masked_fill(~seen, -math.inf)
@@ -311,6 +311,66 @@ def test_decode(device, page, heads, kv, dk, dv, lens, form):
     near(got, want, tol)
 
 
+PROMPT = [  # page, heads, kv heads, dk, dv, lengths, new tokens
+    (64, 8, 1, 128, 128, [700], [700]),
+    (64, 32, 4, 128, 128, [300, 1, 17, 640], [300, 1, 17, 5]),
+    (16, 4, 4, 64, 64, [200, 129, 1000], [200, 64, 2]),
+    (64, 16, 2, 256, 256, [260, 30], [260, 30]),
+    (8, 10, 2, 80, 112, [131, 64], [100, 64]),
+    (32, 24, 2, 96, 160, [257, 64, 0], [7, 64, 0]),
+    (64, 6, 2, 192, 128, [400], [33]),
+    (64, 40, 1, 64, 256, [513], [4]),
+    (16, 5, 1, 16, 16, [90, 300], [90, 150]),
+    (64, 8, 2, 128, 128, [6000], [3]),
+]
+
+
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("page,heads,kv,dk,dv,lens,new", PROMPT)
+@pytest.mark.parametrize("form", ["plain", "window", "cap", "sink", "all"])
+def test_prompt(device, page, heads, kv, dk, dv, lens, new, form):
+    cache, table = filled(lens, page, kv, dk, dv, seed=17, device=device)
+    q = (randn(sum(new), heads, dk, seed=18) * 1.5).bfloat16()
+    more = {"plain": {}, "window": {"window": 100}, "cap": {"softcap": 5.0}, "sink": {"sink": randn(heads, seed=9) * 2},
+            "all": {"window": 33, "softcap": 20.0, "sink": randn(heads, seed=9)}}[form]
+    want, tol, _ = attend(q, cache, table, lens, new, dk ** -0.5, **more)
+    if "sink" in more:
+        more["sink"] = more["sink"].to(device)
+    got = ops.kv8_attention(q.to(device), cache, i32(table, device), i32(lens, device), i32(cum(new), device), max(new), dk ** -0.5, **more)
+    assert status(device) == 0
+    near(got, want, tol)
+
+
+@pytest.mark.parametrize("device", WHERE)
+def test_prompt_rows_apart(device):
+    lens, new, heads, kv, D = [200, 77, 300], [20, 0, 150], 8, 2, 64
+    cache, table = filled(lens, 32, kv, D, D, seed=1, device=device)
+    for shift in (0, 1):
+        wide = randn(170, heads * D + 100 + shift, seed=2).bfloat16().to(device)
+        q = wide[:, shift:shift + heads * D].view(170, heads, D)
+        out = torch.full((172, heads * D + 24 + shift), 7.0, dtype=torch.bfloat16, device=device)
+        mine = out[1:171, 8:8 + heads * D].unflatten(1, (heads, D))
+        ops.kv8_attention(q, cache, i32(table, device), i32(lens, device), i32(cum(new), device), 150, 0.125, max_ctx=300, out=mine)
+        want, tol, _ = attend(q.cpu(), cache, table, lens, new, 0.125)
+        near(mine, want, tol)
+        mine.fill_(7.0)
+        assert bool((out == 7.0).all()) and status(device) == 0
+
+
+@pytest.mark.parametrize("device", WHERE)
+def test_prompt_propagates_nan_to_rows_that_see_it(device):
+    lens, new = [300, 140], [300, 100]
+    cache, table = filled(lens, 16, 1, 64, 64, seed=3, device=device)
+    cache.v.view(torch.uint8)[table[0][9], 0, 5, 9] = NAN          # position 149
+    cache.k.view(torch.uint8)[table[1][6], 0, 7, 0] = NAN          # position 103
+    q = randn(400, 4, 64, seed=4).bfloat16()
+    q[350, 1, 3] = math.nan
+    want, tol, _ = attend(q, cache, table, lens, new, 0.125)
+    assert bool(want[149:300, :, 9].isnan().all()) and not bool(want[:149].isnan().any())
+    got = ops.kv8_attention(q.to(device), cache, i32(table, device), i32(lens, device), i32(cum(new), device), 300, 0.125)
+    near(got, want, tol)
+
+
 @pytest.mark.parametrize("device", WHERE)
 def test_decode_rows_apart(device):
     """Queries cut out of a projection, an output with rows of its own pitch, sequences without a row, max_ctx."""
@@ -333,8 +393,6 @@ def test_decode_rows_apart(device):
 @pytest.mark.parametrize("new", [[1, 1, 1], [9, 1, 30]])
 def test_attention_does_not_see_masked_garbage(device, new):
     """NaN codes and odd scales behind a sequence and in front of its window."""
-    if device != "cpu" and max(new) > 1:
-        pytest.skip("prompt kernel")
     lens, window = [150, 70, 400], 40
     cache, table = filled(lens, 16, 2, 64, 64, seed=3, device=device)
     q = randn(sum(new), 4, 64, seed=4).bfloat16()
