@@ -4,6 +4,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
+
 #include "kv8.h"
 
 namespace {
@@ -52,6 +54,16 @@ void one_device(const Tensor& x, std::initializer_list<const Tensor*> all, const
   LB_ASK(x.is_cuda(), who, ": CUDA tensors");
 }
 
+// sums of weights: a row of their own for every sequence and head
+void check_sums(const Tensor& w, int64_t n, int64_t heads, const char* who) {
+  LB_ASK(w.dim() == 3 && w.scalar_type() == at::kFloat && w.size(0) == n && w.size(1) == heads && (w.stride(2) == 1 || w.size(2) <= 1) &&
+             w.size(2) < (int64_t(1) << 31), who, ": sums of weights are float32 [sequences, kv heads, keys]");
+  const int64_t L = w.size(2), a = w.stride(0), b = w.stride(1);
+  const bool apart = n <= 1 ? (heads <= 1 || b >= L)
+                            : heads <= 1 ? a >= L : (b >= L && a >= (heads - 1) * b + L) || (a >= L && b >= (n - 1) * a + L);
+  LB_ASK(apart, who, ": rows of the sums of weights overlap");
+}
+
 void kv8_append(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& new_k, const Tensor& new_v,
                 const Tensor& table, const Tensor& ctx, const Tensor& cu, int64_t max_new, const Tensor& status) {
   const char* who = "kv8_append";
@@ -70,7 +82,8 @@ void kv8_append(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor
 
 void kv8_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& table,
                    const Tensor& ctx, const Tensor& cu, int64_t max_new, double scale, int64_t window, double softcap, const OptT& sink,
-                   int64_t per, int64_t n_splits, Tensor& out, const Tensor& status) {
+                   int64_t per, int64_t n_splits, Tensor& out, const Tensor& status, const OptT& weights, int64_t observe, int64_t w_per,
+                   int64_t w_splits) {
   const char* who = "kv8_attention";
   const auto c = cache_of(k, v, ks, vs, who);
   LB_ASK(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.stride(2) == 1 && q.size(2) == c.dk, who,
@@ -89,20 +102,64 @@ void kv8_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
     a.sink = sink->data_ptr<float>();
   }
   const auto s = seqs_of(table, ctx, cu, max_new, T, status, who);
+  if (weights.has_value()) {
+    check_sums(*weights, s.n, c.Hkv, who);
+    LB_ASK(weights->device() == q.device() && observe >= 0 && observe < (int64_t(1) << 31) && w_per >= 1 && w_splits >= 1 && w_splits <= 65535,
+           who, ": sums of weights on the queries' device, observed rows not negative");
+  }
   one_device(q, {&k, &v, &ks, &vs, &table, &ctx, &cu, &out, &status}, who);
   c10::cuda::CUDAGuard guard(q.device());
   if (T == 0 || s.n == 0 || max_new == 0) return;
   LB_ASK(per >= 1 && n_splits >= 1 && n_splits <= 128 && n_splits * c.Hkv <= 65535 && T * Hq < (int64_t(1) << 31), who, ": splits, rows");
   Tensor part;
   if (n_splits > 1) part = at::empty({T * Hq * n_splits * (c.dv + 2)}, q.options().dtype(at::kFloat));
+  Tensor lse;
+  if (weights.has_value()) {
+    lse = at::empty({T * Hq}, q.options().dtype(at::kFloat));
+    a.lse = lse.data_ptr<float>();
+  }
   float* pp = n_splits > 1 ? part.data_ptr<float>() : nullptr;
   const int rc = max_new == 1 ? lb::kv8_decode_launch(c, s, a, int(per), int(n_splits), pp, cur_stream())
                               : lb::kv8_prompt_launch(c, s, a, int(n_splits), pp, cur_stream());
   TORCH_CHECK(rc == 0, "kv8_attention: ", lb::kv8_last_error());
+  if (weights.has_value())
+    TORCH_CHECK(lb::kv8_weights_launch(c, s, a, int(observe), int(w_per), int(w_splits), weights->data_ptr<float>(), long(weights->stride(0)),
+                                       long(weights->stride(1)), int(weights->size(2)), cur_stream()) == 0,
+                "kv8_attention: ", lb::kv8_last_error());
+}
+
+void kv8_evict(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& table, const Tensor& ctx,
+               const Tensor& weights, int64_t budget, int64_t first, int64_t last, const Tensor& dst, Tensor& lens, Tensor& kept,
+               Tensor& w_out, const Tensor& status) {
+  const char* who = "kv8_evict";
+  const auto c = cache_of(k, v, ks, vs, who);
+  LB_ASK(table.dim() == 2 && table.scalar_type() == at::kInt && (table.stride(1) == 1 || table.size(1) <= 1) && dst.dim() == 2 &&
+             dst.scalar_type() == at::kInt && (dst.stride(1) == 1 || dst.size(1) <= 1) && dst.size(0) == table.size(0), who,
+         ": block tables are int32 [sequences, blocks]");
+  const int64_t n = table.size(0);
+  LB_ASK(ctx.dim() == 1 && ctx.scalar_type() == at::kInt && ctx.is_contiguous() && ctx.numel() == n, who, ": lengths are int32 [sequences]");
+  LB_ASK(n <= 65535 && table.size(1) < (int64_t(1) << 31) / 64, who, ": at most 65535 sequences");
+  LB_ASK(budget >= 1 && budget < (int64_t(1) << 30) && first >= 0 && last >= 0 && first + last <= budget, who,
+         ": the budget holds the first and last tokens that stay");
+  LB_ASK(dst.size(1) * c.page >= budget, who, ": the blocks of the result hold fewer tokens than the budget");
+  check_sums(weights, n, c.Hkv, who);
+  for (const Tensor* t : {&kept, &w_out})
+    LB_ASK(t->dim() == 3 && t->is_contiguous() && t->size(0) == n && t->size(1) == c.Hkv && t->size(2) == budget, who, ": results");
+  LB_ASK(lens.scalar_type() == at::kInt && kept.scalar_type() == at::kInt && w_out.scalar_type() == at::kFloat && lens.numel() == n &&
+             lens.is_contiguous(), who, ": results");
+  one_device(k, {&v, &ks, &vs, &table, &ctx, &weights, &dst, &lens, &kept, &w_out, &status}, who);
+  c10::cuda::CUDAGuard guard(k.device());
+  const lb::Kv8Seqs s{table.data_ptr<int>(), long(table.stride(0)), int(table.size(1)), ctx.data_ptr<int>(), nullptr, int(n), 0, 0,
+                      static_cast<int*>(status.data_ptr())};
+  const lb::Kv8Evict e{weights.data_ptr<float>(), long(weights.stride(0)), long(weights.stride(1)), int(weights.size(2)), int(budget),
+                       int(first), int(last), dst.data_ptr<int>(), long(dst.stride(0)), lens.data_ptr<int>(), kept.data_ptr<int>(),
+                       w_out.data_ptr<float>()};
+  TORCH_CHECK(lb::kv8_evict_launch(c, s, e, cur_stream()) == 0, "kv8_evict: ", lb::kv8_last_error());
 }
 }  // namespace
 
 void bind_kv8(pybind11::module_& m) {
   m.def("kv8_append", &kv8_append);
   m.def("kv8_attention", &kv8_attention);
+  m.def("kv8_evict", &kv8_evict);
 }

@@ -46,6 +46,22 @@ int kv8_decode_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int
 int kv8_prompt_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int n_splits, float* part, cudaStream_t st);
 // Joins the partial results of every row and head of a prompt call.
 cudaError_t kv8_join(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int n_splits, float* part, cudaStream_t st);
+// w[sequence, kv head, key] += softmax weights of the sequence's last `observe` rows (0: all), with a.lse from the attention; key
+// tiles in n_splits CTAs of `per`.
+int kv8_weights_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int observe, int per, int n_splits, float* w, long w_seq,
+                       long w_head, int w_keys, cudaStream_t st);
+
+// Eviction: of every sequence and kv head the first `first` tokens, the last `last` and those of the largest weights stay, `budget`
+// in all, in order, in the blocks of dst. s.cu and s.max_new are not used.
+struct Kv8Evict {
+  const float* w; long w_seq, w_head; int w_keys;
+  int budget, first, last;
+  const int* dst; long ld_dst;
+  int* lens;                            // [sequences]
+  int* kept;                            // [sequences, kv heads, budget], -1 behind the last
+  float* w_out;                         // likewise, 0 behind the last
+};
+int kv8_evict_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Evict& e, cudaStream_t st);
 const char* kv8_last_error();
 void kv8_set_error(const char* what);
 

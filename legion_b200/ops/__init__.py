@@ -11,7 +11,7 @@ import torch
 
 from . import reference as _ref
 from . import sm100 as _sm
-from .kv8 import Kv8Cache, kv8_append, kv8_attention
+from .kv8 import Kv8Cache, kv8_append, kv8_attention, kv8_evict
 
 reference = _ref
 sm100 = _sm

@@ -55,6 +55,11 @@ def _check(cache: Kv8Cache, who: str):
             raise ValueError(f"{who}: scales are float32 [blocks, kv heads]")
 
 
+def _check_weights(w, cache: Kv8Cache, block_table, who: str):
+    if w.dim() != 3 or w.dtype != torch.float32 or w.shape[:2] != (block_table.shape[0], cache.k.shape[1]):
+        raise ValueError(f"{who}: sums of weights are float32 [sequences, kv heads, keys]")
+
+
 def kv8_append(cache: Kv8Cache, k, v, block_table, ctx_lens, cu_q, max_q_len: int) -> None:
     """Writes the rows' keys and values (``k`` [T, kv heads, dk], ``v`` [T, kv heads, dv], rows and heads may lie apart) to the
     cache. A block that gets its first cell begins anew: its other cells become zero. In others the scale grows where a new value
@@ -90,21 +95,35 @@ def _prompt_splits(n: int, kv_heads: int, rows: int, row_tile: int, tiles: int) 
     return best
 
 
+@functools.lru_cache(maxsize=4096)
+def _weight_split(n: int, kv_heads: int, tiles: int) -> Tuple[int, int]:
+    """(key tiles of a CTA, CTAs of a sequence and head) for the sums of weights: two CTAs an SM."""
+    s = max(1, min(tiles, -(-4 * _sm.NUM_SMS // (n * kv_heads))))
+    per = -(-tiles // s)
+    return per, -(-tiles // per)
+
+
 def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: int, scale: float, window: int = 0, softcap: float = 0.0,
                   sink=None, weights=None, observe: int = 0, max_ctx: Optional[int] = None, out=None):
     """Causal attention of the query rows ``q`` [T, heads, dk] over the cache; returns [T, heads, dv] (``out`` takes it; its rows
     may lie apart). ``window`` > 0: the last that many keys are visible; ``softcap`` > 0: scores become softcap * tanh(score /
     softcap); ``sink`` [heads] float32: exp(sink) joins the denominator. A row that sees no key is zero. ``max_q_len`` == 1 selects
-    the decode kernel. ``max_ctx``: bound of the lengths, for the split over the keys (None: the table's)."""
-    if weights is not None:
-        raise NotImplementedError("kv8_attention: sums of weights")
+    the decode kernel. ``max_ctx``: bound of the lengths, for the split over the keys (None: the table's).
+
+    ``weights`` float32 [sequences, kv heads, >= longest context]: every key's softmax weight, summed over the query heads that
+    share its head and over the sequence's last ``observe`` rows (0: all of the call), is added to its sum: what ``kv8_evict`` goes
+    by. The sums do not depend on the order of anything but the rows."""
     if not q.is_cuda:
         _check(cache, "kv8_attention")
         if q.dim() != 3 or q.shape[2] != cache.k.shape[3] or q.shape[1] % cache.k.shape[1]:
             raise ValueError("kv8_attention: queries [T, heads, head size] do not fit the cache")
         if window < 0 or softcap < 0:
             raise ValueError("kv8_attention: window and soft cap are not negative")
-        o = _ref.kv8_attention(q, cache, block_table, ctx_lens, cu_q, scale, window, softcap, sink)
+        if weights is not None:
+            _check_weights(weights, cache, block_table, "kv8_attention")
+            if observe < 0:
+                raise ValueError("kv8_attention: observed rows are not negative")
+        o = _ref.kv8_attention(q, cache, block_table, ctx_lens, cu_q, scale, window, softcap, sink, weights, observe)
         return o if out is None else out.copy_(o)
     k = cache.k
     if out is None:
@@ -119,6 +138,32 @@ def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: in
     else:
         rows = 256 if k.shape[3] <= 128 and cache.v.shape[3] <= 128 else 128
         per, splits = 1, _prompt_splits(block_table.shape[0], k.shape[1], max_q_len * group, rows, tiles + max_q_len // 128)
+    w_per, w_splits = (1, 1) if weights is None else _weight_split(block_table.shape[0], k.shape[1], max(1, -(-span // 128)))
     _sm.ext().kv8_attention(q, k, cache.v, cache.k_scale, cache.v_scale, block_table, ctx_lens, cu_q, max_q_len, scale, window,
-                            softcap, sink, per, splits, out, _sm.Workspace.get(q.device).status)
+                            softcap, sink, per, splits, out, _sm.Workspace.get(q.device).status, weights, observe, w_per, w_splits)
     return out
+
+
+def kv8_evict(cache: Kv8Cache, block_table, ctx_lens, weights, budget: int, dst_table, keep_first: int = 0, keep_last: int = 0):
+    """Keeps ``budget`` tokens of every sequence and kv head: the first ``keep_first``, the last ``keep_last`` and, of those between,
+    the ones with the largest ``weights`` (as ``kv8_attention`` sums them up; equal ones: the earlier). They move in order to the
+    blocks of ``dst_table`` int32 [sequences, >= budget / page], which no table of the call reads; a sequence that holds no more
+    than the budget moves as it is. Keys keep the rotary positions that they were cached with.
+
+    Returns (lengths int32 [sequences], the kept tokens' places before int32 [sequences, kv heads, budget], -1 behind the last, and
+    their sums float32 likewise, 0 behind the last)."""
+    B, kv = block_table.shape[0], cache.k.shape[1]
+    if not weights.is_cuda:
+        _check(cache, "kv8_evict")
+        _check_weights(weights, cache, block_table, "kv8_evict")
+        if budget < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget or dst_table.shape[0] != B \
+                or dst_table.shape[1] * cache.page < budget:
+            raise ValueError("kv8_evict: the budget holds the first and last tokens that stay, the blocks of the result hold the budget")
+        return _ref.kv8_evict(cache, block_table, ctx_lens, weights, budget, dst_table, keep_first, keep_last)
+    dev = weights.device
+    lens = torch.empty(B, dtype=torch.int32, device=dev)
+    kept = torch.empty(B, kv, max(0, budget), dtype=torch.int32, device=dev)
+    sums = torch.empty(B, kv, max(0, budget), device=dev)
+    _sm.ext().kv8_evict(cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, ctx_lens, weights, budget, keep_first, keep_last,
+                        dst_table, lens, kept, sums, _sm.Workspace.get(dev).status)
+    return lens, kept, sums

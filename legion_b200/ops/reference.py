@@ -693,7 +693,8 @@ def kv8_append(cache, k, v, block_table, ctx_lens, cu_q):
                 at = end
 
 
-def kv8_attention(q, cache, block_table, ctx_lens, cu_q, scale, window: int = 0, softcap: float = 0.0, sink=None):
+def kv8_attention(q, cache, block_table, ctx_lens, cu_q, scale, window: int = 0, softcap: float = 0.0, sink=None, weights=None,
+                  observe: int = 0):
     T, Hq, _ = q.shape
     Hkv, page = cache.k.shape[1], cache.k.shape[2]
     out = q.new_zeros(T, Hq, cache.v.shape[3])
@@ -717,9 +718,42 @@ def kv8_attention(q, cache, block_table, ctx_lens, cu_q, scale, window: int = 0,
             s = torch.cat([s, sink.float().view(Hq, 1, 1).expand(Hq, q1 - q0, 1)], dim=-1)
         p = torch.softmax(s, dim=-1)[..., :ctx]
         p = torch.where(hidden.all(1)[None, :, None], torch.zeros_like(p), p)
+        if weights is not None:
+            seen = p[:, max(0, q1 - q0 - observe) if observe else 0:]
+            weights[i, :, :ctx] += seen.sum(1).view(Hkv, Hq // Hkv, ctx).sum(1)
         bad = v.isnan()                       # a NaN value reaches the rows that see it and no others
         o = torch.einsum("hqk,khd->qhd", p, v.masked_fill(bad, 0.0))
         if bool(bad.any()):
             o = o.masked_fill(torch.einsum("qk,khd->qhd", (~hidden).float(), bad.float()) > 0, float("nan"))
         out[q0:q1] = o.to(q.dtype)
     return out
+
+
+def kv8_evict(cache, block_table, ctx_lens, weights, budget: int, dst_table, keep_first: int = 0, keep_last: int = 0):
+    B, kv = weights.shape[:2]
+    page = cache.k.shape[2]
+    lens = torch.clamp(ctx_lens, min=0, max=budget).to(torch.int32)
+    kept = torch.full((B, kv, budget), -1, dtype=torch.int32, device=weights.device)
+    sums = torch.zeros(B, kv, budget, device=weights.device)
+    for i in range(B):
+        n = int(ctx_lens[i])
+        for h in range(kv):
+            w = weights[i, h, :n]
+            if n <= budget:
+                idx = torch.arange(n, device=w.device)
+            else:
+                mid = torch.sort(w[keep_first:n - keep_last], descending=True, stable=True).indices[:budget - keep_first - keep_last]
+                idx = torch.cat([torch.arange(keep_first, device=w.device), mid.sort().values + keep_first,
+                                 torch.arange(n - keep_last, n, device=w.device)])
+            kept[i, h, :idx.numel()], sums[i, h, :idx.numel()] = idx.to(torch.int32), w[idx]
+            for j in range(0, idx.numel(), page):
+                part, dst = idx[j:j + page], int(dst_table[i, j // page])
+                src = block_table[i].long()[part // page]
+                for codes, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+                    raw, old = codes.view(torch.uint8), scale[src, h]
+                    now = old.max()
+                    x = raw[src, h, part % page].view(codes.dtype).float() * (old / now if now > 0 else torch.zeros_like(old))[:, None]
+                    raw[dst, h] = 0
+                    raw[dst, h, :part.numel()] = x.to(codes.dtype).view(torch.uint8)
+                    scale[dst, h] = now
+    return lens, kept, sums

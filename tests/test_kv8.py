@@ -126,11 +126,12 @@ class Oracle:
 
 
 def attend(q, cache, table, lens, new, scale, window=0, softcap=0.0, sink=None):
-    """(out, tolerance, lse) in float64."""
+    """(out, tolerance, weights [kv heads, keys, rows of the heads that share one] of every sequence, their tolerance) in float64."""
     k_all, v_all = decode(cache.k, cache.k_scale), decode(cache.v, cache.v_scale)
     page, kv = cache.k.shape[2], cache.k.shape[1]
     T, H, D = q.shape
     out, tol = torch.zeros(T, H, v_all.shape[3], dtype=torch.float64), torch.zeros(T, H, v_all.shape[3], dtype=torch.float64)
+    off_w = [torch.zeros(kv, n, H // kv * m, dtype=torch.float64) for n, m in zip(lens, new)]
     weight = [torch.zeros(kv, n, H // kv * m, dtype=torch.float64) for n, m in zip(lens, new)]
     cu = cum(new)
     for i, (n, m) in enumerate(zip(lens, new)):
@@ -162,7 +163,8 @@ def attend(q, cache, table, lens, new, scale, window=0, softcap=0.0, sink=None):
                 least = 2.0 ** -30 * (p[r] * vs).nan_to_num(0, 0, 0).max() * (v / vs[:, None].clamp_min(1e-300))[at].abs().sum(0)
                 tol[cu[i] + r, h] = out[cu[i] + r, h].abs() * 2.0 ** -8 + (2.0 ** -9 + 2 * off) * (p[r, at] @ v[at].abs()) + least
             weight[i][g, :, (h % (H // kv)) * m:(h % (H // kv) + 1) * m] = p.T
-    return out, tol + 1e-30, weight
+            off_w[i][g, :, (h % (H // kv)) * m:(h % (H // kv) + 1) * m] = (2 * off + 2.0 ** -20) * p.T
+    return out, tol + 1e-30, weight, off_w
 
 
 def near(got, want, tol):
@@ -303,7 +305,7 @@ def test_decode(device, page, heads, kv, dk, dv, lens, form):
     more = {"plain": {}, "window": {"window": 100}, "cap": {"softcap": 5.0}, "sink": {"sink": randn(heads, seed=9) * 2},
             "all": {"window": 33, "softcap": 20.0, "sink": randn(heads, seed=9)}}[form]
     new = [1] * len(lens)
-    want, tol, _ = attend(q, cache, table, lens, new, dk ** -0.5, **more)
+    want, tol, _, _ = attend(q, cache, table, lens, new, dk ** -0.5, **more)
     if "sink" in more:
         more["sink"] = more["sink"].to(device)
     got = ops.kv8_attention(q.to(device), cache, i32(table, device), i32(lens, device), i32(cum(new), device), 1, dk ** -0.5, **more)
@@ -333,7 +335,7 @@ def test_prompt(device, page, heads, kv, dk, dv, lens, new, form):
     q = (randn(sum(new), heads, dk, seed=18) * 1.5).bfloat16()
     more = {"plain": {}, "window": {"window": 100}, "cap": {"softcap": 5.0}, "sink": {"sink": randn(heads, seed=9) * 2},
             "all": {"window": 33, "softcap": 20.0, "sink": randn(heads, seed=9)}}[form]
-    want, tol, _ = attend(q, cache, table, lens, new, dk ** -0.5, **more)
+    want, tol, _, _ = attend(q, cache, table, lens, new, dk ** -0.5, **more)
     if "sink" in more:
         more["sink"] = more["sink"].to(device)
     got = ops.kv8_attention(q.to(device), cache, i32(table, device), i32(lens, device), i32(cum(new), device), max(new), dk ** -0.5, **more)
@@ -351,7 +353,7 @@ def test_prompt_rows_apart(device):
         out = torch.full((172, heads * D + 24 + shift), 7.0, dtype=torch.bfloat16, device=device)
         mine = out[1:171, 8:8 + heads * D].unflatten(1, (heads, D))
         ops.kv8_attention(q, cache, i32(table, device), i32(lens, device), i32(cum(new), device), 150, 0.125, max_ctx=300, out=mine)
-        want, tol, _ = attend(q.cpu(), cache, table, lens, new, 0.125)
+        want, tol, _, _ = attend(q.cpu(), cache, table, lens, new, 0.125)
         near(mine, want, tol)
         mine.fill_(7.0)
         assert bool((out == 7.0).all()) and status(device) == 0
@@ -365,7 +367,7 @@ def test_prompt_propagates_nan_to_rows_that_see_it(device):
     cache.k.view(torch.uint8)[table[1][6], 0, 7, 0] = NAN          # position 103
     q = randn(400, 4, 64, seed=4).bfloat16()
     q[350, 1, 3] = math.nan
-    want, tol, _ = attend(q, cache, table, lens, new, 0.125)
+    want, tol, _, _ = attend(q, cache, table, lens, new, 0.125)
     assert bool(want[149:300, :, 9].isnan().all()) and not bool(want[:149].isnan().any())
     got = ops.kv8_attention(q.to(device), cache, i32(table, device), i32(lens, device), i32(cum(new), device), 300, 0.125)
     near(got, want, tol)
@@ -383,7 +385,7 @@ def test_decode_rows_apart(device):
         out = torch.full((4, heads * D + 24), 7.0, dtype=torch.bfloat16, device=device)
         ops.kv8_attention(q, cache, i32(table, device), i32(lens, device), i32(cum(new), device), 1, 0.125, max_ctx=300,
                           out=out[1:3, 8:8 + heads * D].unflatten(1, (heads, D)))
-        want, tol, _ = attend(q.cpu(), cache, table, lens, new, 0.125)
+        want, tol, _, _ = attend(q.cpu(), cache, table, lens, new, 0.125)
         near(out[1:3, 8:8 + heads * D].unflatten(1, (heads, D)), want, tol)
         out[1:3, 8:8 + heads * D] = 7.0
         assert bool((out == 7.0).all()) and status(device) == 0
@@ -396,7 +398,7 @@ def test_attention_does_not_see_masked_garbage(device, new):
     lens, window = [150, 70, 400], 40
     cache, table = filled(lens, 16, 2, 64, 64, seed=3, device=device)
     q = randn(sum(new), 4, 64, seed=4).bfloat16()
-    want, tol, _ = attend(q, cache, table, lens, new, 0.125, window=window)
+    want, tol, _, _ = attend(q, cache, table, lens, new, 0.125, window=window)
     for codes, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
         raw = codes.view(torch.uint8)
         raw[0], scale[0] = NAN, math.nan
@@ -419,7 +421,7 @@ def test_decode_propagates_nan(device):
     cache.k.view(torch.uint8)[table[1][0], 0, 0, 0] = NAN
     q = randn(3, 4, 64, seed=4).bfloat16()
     q[2, 1, 3], q[2, 2, 0] = math.nan, math.inf
-    want, tol, _ = attend(q, cache, table, lens, [1] * 3, 0.125)
+    want, tol, _, _ = attend(q, cache, table, lens, [1] * 3, 0.125)
     want[2, 2] = math.nan                              # an infinite query value: infinity times zero among its products
     got = ops.kv8_attention(q.to(device), cache, i32(table, device), i32(lens, device), i32([0, 1, 2, 3], device), 1, 0.125)
     near(got, want, tol)
@@ -437,9 +439,168 @@ def test_decode_far_apart_scales(device):
     cache = on(cache, device)
     for sharp in (1.0, 30.0):
         q = randn(1, 8, 64, seed=5).mul(sharp).bfloat16()
-        want, tol, _ = attend(q, cache, table, [n], [1], 0.125)
+        want, tol, _, _ = attend(q, cache, table, [n], [1], 0.125)
         got = ops.kv8_attention(q.to(device), cache, i32(table, device), i32([n], device), i32([0, 1], device), 1, 0.125)
         near(got, want, tol)
+
+
+# ---------------------------------------------------------------------------------------- sums of weights, eviction
+WEIGHTS = [  # page, heads, kv heads, dk, dv, lengths, new tokens, observed rows
+    (64, 8, 1, 128, 128, [300, 1, 700], [1, 1, 1], 0),
+    (64, 40, 8, 128, 128, [129, 500], [1, 1], 0),
+    (16, 32, 2, 64, 64, [257, 0, 130], [1, 1, 1], 0),
+    (64, 24, 1, 256, 64, [400], [1], 0),
+    (64, 8, 2, 128, 128, [300, 150], [300, 40], 0),
+    (32, 6, 2, 64, 96, [300, 150, 90], [130, 0, 90], 32),
+    (64, 5, 1, 256, 256, [600], [200], 64),
+    (8, 3, 3, 48, 48, [140], [7], 1),
+    (64, 4, 2, 64, 64, [5000], [3], 2),
+]
+
+
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("page,heads,kv,dk,dv,lens,new,observe", WEIGHTS)
+@pytest.mark.parametrize("form", ["plain", "all"])
+def test_sums_of_weights(device, page, heads, kv, dk, dv, lens, new, observe, form):
+    cache, table = filled(lens, page, kv, dk, dv, seed=27, device=device)
+    q = (randn(sum(new), heads, dk, seed=28) * 1.5).bfloat16()
+    more = {"plain": {}, "all": {"window": 50, "softcap": 20.0, "sink": randn(heads, seed=9)}}[form]
+    _, _, weight, off = attend(q, cache, table, lens, new, dk ** -0.5, **more)
+    if "sink" in more:
+        more["sink"] = more["sink"].to(device)
+    L = max(lens) + 3
+    start = torch.rand(len(lens), kv, L, generator=gen(1))
+    big = torch.full((len(lens), kv + 1, L + 5), -3.0, device=device)
+    w = big[:, 1:, 2:2 + L]
+    w.copy_(start)
+    ops.kv8_attention(q.to(device), cache, i32(table, device), i32(lens, device), i32(cum(new), device), max(new), dk ** -0.5, weights=w,
+                      observe=observe, **more)
+    assert status(device) == 0
+    for i, (n, m) in enumerate(zip(lens, new)):
+        rows = torch.arange(weight[i].shape[2]) % max(m, 1) >= (m - observe if observe else 0)
+        want, tol = weight[i][:, :, rows].sum(2), off[i][:, :, rows].sum(2)
+        got = (w[i].cpu().double() - start[i].double())
+        assert bool(((got[:, :n] - want).abs() <= tol + 2.0 ** -23 * (start[i, :, :n] + want)).all())
+        assert not bool(got[:, n:].any())
+    w.fill_(-3.0)
+    assert bool((big == -3.0).all())
+
+
+def evict(cache, table, lens, w, budget, dst, first, last):
+    """The rules of eviction on code values, in float64: (kept, sums, keys and values by block, scales)."""
+    page = cache.k.shape[2]
+    kept, sums, blocks = [], [], {}
+    for i, n in enumerate(lens):
+        for h in range(w.shape[1]):
+            order = sorted(range(n), key=lambda t: (not (t < first or t >= n - last), -float(w[i, h, t]), t))
+            stay = sorted(order[:budget])
+            kept.append(stay + [-1] * (budget - len(stay)))
+            sums.append([float(w[i, h, t]) for t in stay] + [0.0] * (budget - len(stay)))
+            for j in range(0, len(stay), page):
+                for name in ("k", "v"):
+                    codes, scale = CODES[getattr(cache, name).view(torch.uint8).long()], getattr(cache, name + "_scale").double()
+                    part = stay[j:j + page]
+                    src = [table[i][t // page] for t in part]
+                    now = max(float(scale[s, h]) for s in src)
+                    rows = torch.zeros(page, codes.shape[3], dtype=torch.float64)
+                    for r, (t, s) in enumerate(zip(part, src)):
+                        rows[r] = encode(codes[s, h, t % page] * (float(scale[s, h]) / now if now else 0.0))
+                    blocks[name, dst[i][j // page], h] = rows, now
+    return kept, sums, blocks
+
+
+EVICT = [  # page, kv heads, dk, dv, lengths, budget, first, last
+    (16, 2, 64, 64, [100, 40, 41, 0, 7], 40, 4, 8),
+    (64, 1, 128, 32, [700], 130, 0, 0),
+    (8, 3, 16, 48, [90, 33], 33, 33, 0),
+    (64, 1, 32, 32, [1500], 1, 0, 1),
+    (16, 1, 32, 16, [3000], 1000, 1, 100),
+]
+
+
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("page,kv,dk,dv,lens,budget,first,last", EVICT)
+@pytest.mark.parametrize("weights", ["spread", "equal", "ties", "signed"])
+def test_evict(device, page, kv, dk, dv, lens, budget, first, last, weights):
+    cache, table = filled(lens, page, kv, dk, dv, seed=5)
+    w = torch.exp2(randn(len(lens), kv, max(lens) + 2, seed=6) * 4)
+    if weights == "equal":
+        w = torch.full_like(w, 0.25)
+    elif weights == "ties":
+        w = torch.round(w).clamp(max=3)
+    elif weights == "signed":
+        w = torch.round(randn(*w.shape, seed=8) * 4) / 4
+        w[..., ::7] *= -0.0
+    # block 0 and those behind the sequences' are free
+    n_old, per = cache.k.shape[0], -(-budget // page)
+    dst = (torch.randperm(len(lens) * per, generator=gen(2)) + n_old).view(len(lens), per).tolist()
+    more = ops.Kv8Cache.empty(n_old + len(lens) * per, page, kv, dk, dv)
+    for name in cache.__slots__:
+        getattr(more, name).view(torch.uint8)[:] = 0x7F if name in "kv" else 0
+        a, b = getattr(more, name), getattr(cache, name)
+        (a.view(torch.uint8) if name in "kv" else a)[:n_old] = b.view(torch.uint8) if name in "kv" else b
+    kept, sums, blocks = evict(more, table, lens, w, budget, dst, first, last)
+    got = on(more, device)
+    lens_out, kept_out, sums_out = ops.kv8_evict(got, i32(table, device), i32(lens, device), w.to(device), budget, i32(dst, device), first, last)
+    assert status(device) == 0
+    assert lens_out.tolist() == [min(n, budget) for n in lens]
+    assert kept_out.flatten(0, 1).tolist() == kept
+    assert sums_out.flatten(0, 1).tolist() == sums
+    for name in ("k", "v"):
+        codes = getattr(got, name).cpu().view(torch.uint8)
+        before = getattr(more, name).view(torch.uint8)
+        for blk in range(codes.shape[0]):
+            for h in range(kv):
+                if (name, blk, h) in blocks:
+                    rows, now = blocks[name, blk, h]
+                    assert torch.equal(CODES[codes[blk, h].long()], rows) and float(getattr(got, name + "_scale")[blk, h]) == now
+                else:
+                    assert torch.equal(codes[blk, h], before[blk, h])
+
+
+@pytest.mark.parametrize("device", WHERE)
+def test_a_chat_whose_cache_is_pruned(device):
+    """Append, attend with sums, evict, go on in the new blocks: attention over what stayed equals the float64 form over the kept
+    tokens, and a second eviction counts on."""
+    page, kv, heads, D, budget = 16, 2, 8, 64, 48
+    cache = ops.Kv8Cache.empty(40, page, kv, D, D, device)
+    table = [[1, 2, 3, 4, 5, 6, 7, 8, 0, 0], [11, 12, 13, 14, 15, 16, 17, 18, 0, 0]]
+    sums = torch.zeros(2, kv, 160, device=device)
+    lens, step = [0, 0], 0
+    spare = [[20, 21, 22, 23, 24, 25], [30, 31, 32, 33, 34, 35]]
+
+    def forward(new):
+        nonlocal lens, step
+        lens, step = [a + b for a, b in zip(lens, new)], step + 1
+        T = sum(new)
+        k, v, q = (randn(T, h, D, seed=100 * step + j).bfloat16().to(device) for j, h in enumerate((kv, kv, heads)))
+        args = (i32(table, device), i32(lens, device), i32(cum(new), device), max(new))
+        ops.kv8_append(cache, k, v, *args)
+        before = sums.cpu().double()
+        out = ops.kv8_attention(q, cache, *args, 0.3, weights=sums)
+        want, tol, weight, off = attend(q.cpu(), on(cache, "cpu"), table, lens, new, 0.3)
+        near(out, want, tol)
+        for i, n in enumerate(lens):
+            got = sums[i, :, :n].cpu().double() - before[i, :, :n]
+            assert bool(((got - weight[i].sum(2)).abs() <= off[i].sum(2) + 2.0 ** -22 * (1 + before[i, :, :n])).all())
+
+    forward([100, 70])
+    for _ in range(3):
+        forward([1, 1])
+    for again in range(2):
+        dst = [s[:3] for s in spare]
+        n, kept, w = ops.kv8_evict(cache, i32(table, device), i32(lens, device), sums, budget, i32(dst, device), 2, 10)
+        lens = n.tolist()
+        assert lens == [budget, budget] and kept.shape == (2, kv, budget)
+        old = table
+        table = [d + s[3:] + [0] * 4 for d, s in zip(dst, spare)]
+        spare = [[b for b in o if b][:6] for o in old]
+        sums.zero_()
+        sums[..., :budget] = w
+        forward([1, 1])
+        forward([20, 3])
+        forward([1, 1])
+    assert status(device) == 0
 
 
 # -------------------------------------------------------------------------------------------------------- refusals
@@ -485,10 +646,45 @@ def test_refusals_need_no_gpu(what):
     out = torch.zeros(1, a["q"].shape[1], c.v.shape[3], dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="kv8_attention"):
         C.kv8_attention(a["q"], c.k, c.v, c.k_scale, c.v_scale, a["table"], a["ctx"], a["cu"], 1, 0.1, kw["window"], kw["softcap"], None, 1, 1,
-                        out, st)
+                        out, st, None, 0, 1, 1)
     if what in ("scale type", "int64 lengths", "bounds", "page", "code type", "devices"):
         with pytest.raises(ValueError, match="kv8_append"):
             C.kv8_append(c.k, c.v, c.k_scale, c.v_scale, a["k"], a["k"], a["table"], a["ctx"], a["cu"], 1, st)
+
+
+@pytest.mark.parametrize("what", ["sums type", "sums shape", "rows overlap", "observe", "budget", "first and last", "blocks", "no budget"])
+def test_refusals_of_sums_and_eviction_need_no_gpu(what):
+    if not ops.sm100.have_ext():
+        pytest.skip("extension not built")
+    a = _refusals()()
+    c, C, st = a["cache"], ops.sm100.ext(), torch.zeros(4, dtype=torch.int32)
+    w, observe, budget, first, last, dst = torch.zeros(1, 2, 20), 0, 16, 0, 0, i32([[1, 2]])
+    if what == "sums type":
+        w = w.double()
+    elif what == "sums shape":
+        w = w[:, :1]
+    elif what == "rows overlap":
+        w = torch.zeros(1, 1, 20).expand(1, 2, 20)
+    elif what == "observe":
+        observe = -1
+    elif what == "budget":
+        budget = 40
+    elif what == "first and last":
+        first, last = 10, 7
+    elif what == "blocks":
+        dst = i32([[1, 2], [3, 4]])
+    elif what == "no budget":
+        budget = 0
+    if what in ("sums type", "sums shape", "rows overlap", "observe"):
+        with pytest.raises(ValueError, match="kv8_attention"):
+            C.kv8_attention(a["q"], c.k, c.v, c.k_scale, c.v_scale, a["table"], a["ctx"], a["cu"], 1, 0.1, 0, 0.0, None, 1, 1,
+                            torch.zeros(1, 4, 32, dtype=torch.bfloat16), st, w, observe, 1, 1)
+    if what != "observe":
+        with pytest.raises(ValueError, match="kv8_evict"):
+            C.kv8_evict(c.k, c.v, c.k_scale, c.v_scale, a["table"], a["ctx"], w, budget, first, last, dst, i32([0]),
+                        torch.zeros(1, 2, budget, dtype=torch.int32), torch.zeros(1, 2, budget), st)
+        with pytest.raises(ValueError):
+            ops.kv8_evict(c, a["table"], a["ctx"], w if what != "rows overlap" else w[:, :1], budget, dst, first, last)
 
 
 def test_cpu_refusals():
