@@ -196,19 +196,22 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     if (lane == 0) {
       constexpr uint32_t idesc_s = umma_idesc(128, NS, 0, 0, 0, 0);       // e4m3 x e4m3
       constexpr uint32_t idesc_o = umma_idesc(128, NO, 0, 1, 1, 0);       // e4m3 (V^T, MN-major) x e5m2
-      const uint32_t qa = smem_u32(q_s);
+      // Descriptors are made once; a step adds its offset in 16-byte units. (Made anew for every MMA they take the one issuing
+      // thread 170 clocks each; an MMA of this shape takes 40.)
+      const uint64_t dk = umma_desc_k_sw128(smem_u32(k_s)), dq = umma_desc_k_sw128(smem_u32(q_s));
+      const uint64_t dv = umma_desc_mn_sw128(smem_u32(v_s), BKV * 128, 1024), dp = umma_desc_k_sw128(smem_u32(p_s));
       auto fail = [&](int code) { *abort_flag = 1; atomicCAS(p.s.status, 0, code | SITE_DECODE_ATTN); return false; };
       auto issue_s = [&](int i) -> bool {
         const int st = i % ST;
         if (!mbar_wait(&k_full[st], (i / ST) & 1, abort_flag)) return fail(ST_TIMEOUT_FULL);
         tc_fence_after();
-        const uint32_t ka = smem_u32(k_s + st * C::K_BYTES);
+        const uint64_t da = dk + uint32_t(st) * (C::K_BYTES / 16);
+        const uint32_t ts = tmem_S + (i & 1) * NS;
 #pragma unroll
         for (int h = 0; h < KH; ++h) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_f8(tmem_S + (i & 1) * NS, umma_desc_k_sw128(ka + h * (BKV * 128) + k * 32),
-                    umma_desc_k_sw128(qa + h * (NS * 128) + k * 32), idesc_s, (h | k) ? 1u : 0u);
+            umma_f8(ts, da + (h * (BKV * 8) + k * 2), dq + (h * (NS * 8) + k * 2), idesc_s, (h | k) ? 1u : 0u);
         }
         umma_commit(&s_full[i & 1]);
         umma_commit(&k_empty[st]);
@@ -222,13 +225,13 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!mbar_wait(&p_ready[w], (i >> 1) & 1, abort_flag)) { fail(ST_TIMEOUT_FLAG); break; }
         if (!mbar_wait(&v_full[st], (i / ST) & 1, abort_flag)) { fail(ST_TIMEOUT_FULL); break; }
         tc_fence_after();
-        const uint32_t va = smem_u32(v_s + st * C::V_BYTES), pa = smem_u32(p_s + w * C::P_BYTES);
+        const uint64_t da = dv + uint32_t(st) * (C::V_BYTES / 16), db = dp + uint32_t(w) * (C::P_BYTES / 16);
+        const uint32_t to = tmem_O + w * MT * NO;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
           for (int k = 0; k < BKV / 32; ++k)
-            umma_f8(tmem_O + (w * MT + mt) * NO, umma_desc_mn_sw128(va + mt * (BKV * 128) + k * 32 * 128, BKV * 128, 1024),
-                    umma_desc_k_sw128(pa + k * 32), idesc_o, ((i >> 1) | k) ? 1u : 0u);
+            umma_f8(to + mt * NO, da + (mt * (BKV * 8) + k * 256), db + k * 2, idesc_o, ((i >> 1) | k) ? 1u : 0u);
         }
         umma_commit(&o_done[w]);
         umma_commit(&v_empty[st]);

@@ -63,14 +63,6 @@ __device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t (&r)[32])
       "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-__device__ __forceinline__ void tm_st16p(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
 __device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // packed fp32 pairs and the three-input maximum
@@ -100,7 +92,54 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <int KH, int MT, bool CAP>
+// One row of a tile: w = halves of 2^(z + ref), their sum with every value scale divided out, and the largest z + ref. WIDE: a
+// scale for 32 keys or more, else for 8. MASK: keys outside [lo, hi) of the tile count nothing.
+template <bool MASK, bool CAP, bool WIDE>
+__device__ __forceinline__ void row_of_tile(uint32_t my_S, const float4* sc, float fq, float ref, float cap_scale, int lo, int hi,
+                                            uint32_t (&w)[64], float& top, float& total) {
+  constexpr int PER = WIDE ? 32 : 8;
+  float mx0 = -INFINITY, mx1 = -INFINITY;
+  total = 0.f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    uint32_t r[32];
+    tmem_ld32(my_S + g * 32, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 32; e += PER) {
+      const float4 f = sc[(g * 32 + e) / 8];
+      const float mul = fq * f.x, add = CAP ? f.y + ref + 0.5f * cap_scale : f.y + ref;
+      const uint64_t mul2 = f2(mul, mul), add2 = f2(add, add);
+      uint64_t acc = f2(0.f, 0.f);
+#pragma unroll
+      for (int j = e; j < e + PER; j += 2) {
+        float z0, z1;
+        if constexpr (CAP) {
+          z0 = fmaf(softcap_r(__uint_as_float(r[j]) * mul, 1.f), cap_scale, add);
+          z1 = fmaf(softcap_r(__uint_as_float(r[j + 1]) * mul, 1.f), cap_scale, add);
+        } else {
+          f2_out(f2_fma(f2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), mul2, add2), z0, z1);
+        }
+        if constexpr (MASK) {
+          const int key = g * 32 + j;
+          if (key < lo || key >= hi) z0 = -INFINITY;
+          if (key + 1 < lo || key + 1 >= hi) z1 = -INFINITY;
+        }
+        if (j & 2) mx1 = fmax3(mx1, z0, z1);
+        else mx0 = fmax3(mx0, z0, z1);
+        const float y0 = ex2(z0), y1 = ex2(z1);
+        acc = f2_add(acc, f2(y0, y1));
+        w[(g * 32 + j) / 2] = half2_of(y0, y1);
+      }
+      float a0, a1;
+      f2_out(acc, a0, a1);
+      total = fmaf(a0 + a1, f.z, total);
+    }
+  }
+  top = fmaxf(mx0, mx1);
+}
+
+template <int KH, int MT, bool CAP, bool WIDE>
 __global__ void __launch_bounds__(PCfg<KH, MT>::THREADS, 1)
 kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PromptArgs p) {
   using C = PCfg<KH, MT>;
@@ -244,20 +283,24 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       // ---------------------------------------------------------------- MMA
       constexpr uint32_t idesc_s = umma_idesc(128, BKV, 0, 0, 0, 0);            // e4m3 x e4m3
       constexpr uint32_t idesc_o = umma_idesc(128, MT * 128, 0, 0, 0, 1);       // half x half, V is MN-major
-      const uint32_t qa = smem_u32(q_s), ka0 = smem_u32(k_s), va0 = smem_u32(v16_s);
+      // descriptors are made once; a step adds its offset in 16-byte units (made anew for every MMA they took the issuing thread
+      // twice as long as the MMAs)
+      const uint64_t dq = umma_desc_k_sw128(smem_u32(q_s)), dk = umma_desc_k_sw128(smem_u32(k_s));
+      const uint64_t dv = umma_desc_mn_sw128(smem_u32(v16_s), 16384, 1024);
       const int units = n_tiles * n_rt;
       auto issue_s = [&](int u) -> bool {
         const int i = u / n_rt, r = u % n_rt, st = i % KS;
         if (!mbar_wait(&k_full[st], (i / KS) & 1, abort_flag)) return fail(ST_TIMEOUT_FULL);
         tc_fence_after();
+        const uint64_t da = dq + uint32_t(r) * (2 * KH * 1024), db = dk + uint32_t(st) * (C::K_BYTES / 16);
+        const uint32_t ts = tmem + (u & 1) * 128;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
           for (int h = 0; h < KH; ++h) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_f8(tmem + (u & 1) * 128, umma_desc_k_sw128(qa + ((r * 2 + t) * KH + h) * 16384 + k * 32),
-                      umma_desc_k_sw128(ka0 + st * C::K_BYTES + h * 16384 + k * 32), idesc_s, (t | h | k) ? 1u : 0u);
+              umma_f8(ts, da + ((t * KH + h) * 1024 + k * 2), db + (h * 1024 + k * 2), idesc_s, (t | h | k) ? 1u : 0u);
           }
         }
         umma_commit(&s_full[u & 1]);
@@ -272,10 +315,10 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!mbar_wait(&v16_full[st], (i / V16S) & 1, abort_flag)) { fail(ST_TIMEOUT_FULL); break; }
         if (!mbar_wait(&p_ready[u & 1], (u >> 1) & 1, abort_flag)) { fail(ST_TIMEOUT_FLAG); break; }
         tc_fence_after();
+        const uint64_t db = dv + uint32_t(st) * (C::V16_BYTES / 16);
+        const uint32_t to = tmem + C::O_COL + r * (MT * 128), ta = tmem + (u & 1) * 128;
 #pragma unroll
-        for (int k = 0; k < BKV / 16; ++k)
-          umma_f16_ts(tmem + C::O_COL + r * (MT * 128), tmem + (u & 1) * 128 + k * 8,
-                      umma_desc_mn_sw128(va0 + st * C::V16_BYTES + k * 16 * 128, 16384, 1024), idesc_o, (i | k) ? 1u : 0u);
+        for (int k = 0; k < BKV / 16; ++k) umma_f16_ts(to, ta + k * 8, db + k * 128, idesc_o, (i | k) ? 1u : 0u);
         umma_commit(&o_done[u & 1]);
         if (r == n_rt - 1) umma_commit(&v16_empty[st]);
         if (u + 2 < units && !issue_s(u + 2)) break;
@@ -297,37 +340,39 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const bool seen = tok >= key_lo && tok < key_hi;      // the others may hold anything: zeros
       const uint8_t* src = v8_s + v8 * C::V8_BYTES + key * 128;
       uint8_t* dst = v16_s + v16 * C::V16_BYTES + key * 128;
-#pragma unroll
+#pragma unroll 1
       for (int h = 0; h < MT; ++h) {
+        uint32_t x[32];
+        uint32_t any = 0;
 #pragma unroll
         for (int ch = 0; ch < 8; ++ch) {
           uint4 w = make_uint4(0u, 0u, 0u, 0u);
           if (seen) w = *reinterpret_cast<const uint4*>(src + h * 16384 + ((ch ^ (key & 7)) << 4));
+          x[4 * ch] = w.x; x[4 * ch + 1] = w.y; x[4 * ch + 2] = w.z; x[4 * ch + 3] = w.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) any |= (x[j] & 0x7f7f7f7fu) + 0x01010101u;
+        if (any & 0x80808080u) {
           // NaN codes: noted (rows that see one become NaN at the end), and not multiplied with the zeros of rows that do not
-          const uint32_t any = (((w.x & 0x7f7f7f7fu) + 0x01010101u) | ((w.y & 0x7f7f7f7fu) + 0x01010101u) |
-                                ((w.z & 0x7f7f7f7fu) + 0x01010101u) | ((w.w & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u;
-          if (any) {
-            atomicMin(&s_nan[0], tok);
-            atomicMax(&s_nan[1], tok);
-            uint32_t* ww = &w.x;
+          atomicMin(&s_nan[0], tok);
+          atomicMax(&s_nan[1], tok);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if (((ww[j] >> (8 * e)) & 0x7fu) == 0x7fu) {
-                  const int d = h * 128 + ch * 16 + j * 4 + e;
-                  atomicOr(&s_nan[2 + d / 32], 1 << (d & 31));
-                  ww[j] &= ~(0xffu << (8 * e));
-                }
+          for (int j = 0; j < 32; ++j) {
+            for (int e = 0; e < 4; ++e) {
+              if (((x[j] >> (8 * e)) & 0x7fu) == 0x7fu) {
+                atomicOr(&s_nan[2 + h * 4 + j / 8], 1 << (4 * (j % 8) + e));
+                x[j] &= ~(0xffu << (8 * e));
               }
             }
           }
+        }
+#pragma unroll
+        for (int ch = 0; ch < 8; ++ch) {
           uint32_t o[8];
-          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const __half2 x = e4m3x2_to_half2(ws[j / 2] >> (16 * (j & 1)));
-            o[j] = *reinterpret_cast<const uint32_t*>(&x);
+            const __half2 y = e4m3x2_to_half2(x[4 * ch + j / 2] >> (16 * (j & 1)));
+            o[j] = *reinterpret_cast<const uint32_t*>(&y);
           }
           uint8_t* d8 = dst + (h * 2 + ch / 4) * 16384;
           const int c0 = (ch % 4) * 2;
@@ -419,84 +464,47 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const int key0 = (tile0 + i) * BKV;
         // entirely visible to every row of the CTA: no masks
         const bool full = rows == RT * 128 && key0 + BKV <= min(ctx, pos_first + 1) && (p.a.window == 0 || key0 > pos_last - p.a.window);
-        auto z_of = [&](uint32_t s, float mul, float add) -> float {
-          float x = __uint_as_float(s) * mul;
-          if constexpr (CAP) return fmaf(softcap_r(x, 1.f), p.scale_log2, 0.5f * p.scale_log2 + add);
-          return x + add;
-        };
-        float mx = -INFINITY;
+        // With the reference as it stands; where a row's largest passes it by more than the slack (in the first tile, and rarely
+        // after it), the references move, O and l follow, and the tile is taken again: its scores are still there.
+        uint32_t w[64];
+        float top, total;
 #pragma unroll 1
-        for (int g = 0; g < 4; ++g) {
-          uint32_t r[32];
-          tmem_ld32(my_S + g * 32, r);
-          tmem_ld_wait();
+        for (int again = 0;; ++again) {
+          const float ref = m == -INFINITY ? 0.f : P_OFFSET - m;
+          if (full) row_of_tile<false, CAP, WIDE>(my_S, sc, fq, ref, p.scale_log2, 0, 0, w, top, total);
+          else row_of_tile<true, CAP, WIDE>(my_S, sc, fq, ref, p.scale_log2, lo - key0, hi - key0, w, top, total);
+          const bool over = m == -INFINITY ? top > -INFINITY : top > P_OFFSET + P_SLACK;
+          if (again || !__any_sync(0xffffffffu, over)) break;
+          float alpha = 1.f;
+          if (over) {
+            const float now = top - ref;
+            alpha = ex2(m - now);                  // (0 at first)
+            m = now;
+          }
+          l *= alpha;
+          if (i > 0) {
+            // O may be touched once P V of the tile before is done: with two row tiles it ran before these scores, with one it may
+            // not have
+            if (n_rt == 1 && !__all_sync(0xffffffffu, mbar_wait(&o_done[(u - 1) & 1], ((u - 1) >> 1) & 1, abort_flag))) {
+              ok = fail(ST_TIMEOUT_TMEM_EMPTY);
+              break;
+            }
+            tc_fence_after();
+#pragma unroll 1
+            for (int d = 0; d < MT * 128; d += 32) {
+              uint32_t r[32];
+              tmem_ld32(my_O + d, r);
+              tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float4 f = sc[g * 4 + e];
-            const float mul = fq * f.x;
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-              const int key = key0 + g * 32 + e * 8 + j;
-              float z0 = z_of(r[e * 8 + j], mul, f.y), z1 = z_of(r[e * 8 + j + 1], mul, f.y);
-              if (!full) {
-                if (key < lo || key >= hi) z0 = -INFINITY;
-                if (key + 1 < lo || key + 1 >= hi) z1 = -INFINITY;
-              }
-              mx = fmax3(mx, z0, z1);
+              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
+              tm_st32(my_O + d, r);
             }
           }
         }
-        float alpha = 1.f;
-        if (mx > m + P_SLACK) {
-          alpha = m == -INFINITY ? 0.f : ex2(m - mx);
-          m = mx;
-        }
-        l *= alpha;
-        if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-          // O may be touched once P V of the tile before is done: with two row tiles it ran before these scores, with one it may not have
-          if (n_rt == 1 && !__all_sync(0xffffffffu, mbar_wait(&o_done[(u - 1) & 1], ((u - 1) >> 1) & 1, abort_flag))) {
-            fail(ST_TIMEOUT_TMEM_EMPTY);
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-#pragma unroll 1
-          for (int d = 0; d < MT * 128; d += 32) {
-            uint32_t r[32];
-            tmem_ld32(my_O + d, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
-            tm_st32(my_O + d, r);
-          }
-        }
-        const float ref = m == -INFINITY ? 0.f : P_OFFSET - m;
-#pragma unroll 1
-        for (int g = 0; g < 4; ++g) {
-          uint32_t r[32], w[16];
-          tmem_ld32(my_S + g * 32, r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float4 f = sc[g * 4 + e];
-            const float mul = fq * f.x;
-            float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-              const int key = key0 + g * 32 + e * 8 + j;
-              float y0 = ex2(z_of(r[e * 8 + j], mul, f.y + ref)), y1 = ex2(z_of(r[e * 8 + j + 1], mul, f.y + ref));
-              if (!full) {
-                if (key < lo || key >= hi) y0 = 0.f;
-                if (key + 1 < lo || key + 1 >= hi) y1 = 0.f;
-              }
-              sum0 += y0;
-              sum1 += y1;
-              w[e * 4 + j / 2] = half2_of(y0, y1);
-            }
-            l = fmaf(sum0 + sum1, f.z, l);
-          }
-          tm_st16p(my_S + g * 16, w);
-        }
+        if (!ok) break;
+        tm_st32(my_S, *reinterpret_cast<uint32_t(*)[32]>(w));
+        tm_st32(my_S + 32, *reinterpret_cast<uint32_t(*)[32]>(w + 32));
+        l += total;                                // (once per tile: thousands of single additions would cost it 2^-20)
         tm_st_wait();
         tc_fence_before();
         mbar_arrive(&p_ready[b]);
@@ -571,10 +579,10 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   }
 }
 
-template <int KH, int MT, bool CAP>
+template <int KH, int MT, bool CAP, bool WIDE>
 cudaError_t launch(const CUtensorMap* tk, const CUtensorMap* tv, const PromptArgs& p, cudaStream_t st) {
   using C = PCfg<KH, MT>;
-  auto kfn = kv8_prompt_kernel<KH, MT, CAP>;
+  auto kfn = kv8_prompt_kernel<KH, MT, CAP, WIDE>;
   static DeviceOnce once;
   const cudaError_t e = once.shared_memory(reinterpret_cast<const void*>(kfn), C::SMEM);
   if (e != cudaSuccess) return e;
@@ -603,8 +611,11 @@ int kv8_prompt_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int
   }
   const int kh = (c.dk + 127) / 128, mt = (c.dv + 127) / 128;
   cudaError_t e = cudaErrorInvalidValue;
-#define LB_KV8(K_, V_) \
-  if (kh == K_ && mt == V_) e = cap ? launch<K_, V_, true>(tk, tv, p, st) : launch<K_, V_, false>(tk, tv, p, st);
+  const bool wide = c.page >= 32;
+#define LB_KV8(K_, V_)                                                                                                          \
+  if (kh == K_ && mt == V_)                                                                                                     \
+    e = cap ? (wide ? launch<K_, V_, true, true>(tk, tv, p, st) : launch<K_, V_, true, false>(tk, tv, p, st))                   \
+            : (wide ? launch<K_, V_, false, true>(tk, tv, p, st) : launch<K_, V_, false, false>(tk, tv, p, st));
   LB_KV8(1, 1) LB_KV8(1, 2) LB_KV8(2, 1) LB_KV8(2, 2)
 #undef LB_KV8
   if (e == cudaSuccess && n_splits > 1) e = kv8_join(c, s, a, n_splits, part, st);

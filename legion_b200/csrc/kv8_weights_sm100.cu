@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
   } else if (warp == 8) {
     if (lane == 0) {
       constexpr uint32_t idesc = umma_idesc(128, NS, 0, 0, 0, 0);
-      const uint32_t qa = smem_u32(q_s), ka0 = smem_u32(k_s);
+      const uint64_t dk = umma_desc_k_sw128(smem_u32(k_s)), dq = umma_desc_k_sw128(smem_u32(q_s));
       bool ok = true;
       int it = 0, staged = 0;
       for (int rt = 0; ok && rt < n_rt; ++rt) {
@@ -154,12 +154,12 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
           ok = (it < 2 || mbar_wait(&s_empty[b], ((it >> 1) - 1) & 1, abort_flag)) && mbar_wait(&k_full[st], (it / ST) & 1, abort_flag);
           if (!ok) { fail(ST_TIMEOUT_FULL); break; }
           tc_fence_after();
+          const uint64_t da = dk + uint32_t(st) * (C::K_BYTES / 16);
 #pragma unroll
           for (int h = 0; h < KH; ++h) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_f8(tmem + b * NS, umma_desc_k_sw128(ka0 + st * C::K_BYTES + h * 16384 + k * 32),
-                      umma_desc_k_sw128(qa + h * (NS * 128) + k * 32), idesc, (h | k) ? 1u : 0u);
+              umma_f8(tmem + b * NS, da + (h * 1024 + k * 2), dq + (h * (NS * 8) + k * 2), idesc, (h | k) ? 1u : 0u);
           }
           umma_commit(&s_full[b]);
           umma_commit(&k_empty[st]);
