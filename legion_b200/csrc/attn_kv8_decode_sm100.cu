@@ -13,8 +13,9 @@
 // the denominator adds exp(z) 2^-e.
 //
 // Two softmax warpgroups (warps 0..3 and 4..7; thread = key of the tile, later output column) take alternate tiles, each a
-// stream of its own with its S^T, P and O^T; they meet in shared memory at the end. Warp 8: MMAs, scores two tiles ahead of
-// their softmax. Warp 9: TMA through the block table into as many stages as 192 KB hold (six of 32 KB for heads of 128), which
+// stream of its own with its P and O^T; they meet in shared memory at the end. Warp 8: MMAs, scores four tiles ahead of
+// their softmax (a wait for a phase of a stage's barrier cannot miss it: the stage's next scores stand behind P of this tile, the
+// stage's next P V behind P of the tile that waits). Warp 9: TMA through the block table into as many stages as 192 KB hold (six of 32 KB for heads of 128), which
 // is what a memory-bound kernel needs in flight. Splits of a sequence write partial results for kv8_combine_kernel; a split
 // covers the same number of tiles in every sequence, so CTAs of a ragged batch are alike. Scratch belongs to the call.
 #include "kv8_dev.cuh"
@@ -32,8 +33,11 @@ struct DecodeArgs {
   float* part;                  // [T][Hq][n_splits][dv + 2]: sums over the values, reference (log2), denominator
 };
 
-constexpr float OFFSET = 13.f;         // P is taken relative to the reference times 2^13: a half reaches 2^37 below its largest
-constexpr float SLACK = 2.f;           // the reference moves when a score passes it by 2^2: 2^15 still fits e5m2
+// P is taken relative to the reference times 2^11, and the reference moves when a weight passes it by more than 2^4: at most 2^15,
+// which e5m2 and a half hold, and e5m2's last step, 2^-16, lies 2^-27 below the largest weight. (A reference within 2^2 moved in a
+// quarter of the tiles of a stream of 2000 keys, 1900 clocks each.)
+constexpr float OFFSET = 11.f;
+constexpr float SLACK = 4.f;
 
 __device__ __forceinline__ int ordered(float f) {
   const int i = __float_as_int(f);
@@ -71,16 +75,17 @@ struct Cfg {
   static constexpr int O_BYTES = NQ * MT * 128 * 4;                        // the second warpgroup's sums on their way to the first
   static constexpr int TAIL = 1024;
   static constexpr int SMEM = STAGES * (K_BYTES + V_BYTES) + Q_BYTES + 2 * P_BYTES + TAIL + 1024;
-  static constexpr int TMEM_RAW = 2 * NS + 2 * MT * NO;
-  static constexpr int TMEM_COLS = TMEM_RAW <= 128 ? 128 : 256;
-  static_assert(TMEM_RAW <= 256 && SMEM <= 227 * 1024 && O_BYTES <= K_BYTES, "sizes");
+  static constexpr int LA = STAGES < 4 ? STAGES : 4;                       // tiles whose scores are made ahead
+  static constexpr int TMEM_RAW = LA * NS + 2 * MT * NO;
+  static constexpr int TMEM_COLS = TMEM_RAW <= 128 ? 128 : TMEM_RAW <= 256 ? 256 : 512;
+  static_assert(TMEM_RAW <= 512 && STAGES >= 3 && STAGES <= 6 && SMEM <= 227 * 1024 && O_BYTES <= K_BYTES, "sizes");
 };
 
 template <int KH, int MT, int NQ, bool CAP>
 __global__ void __launch_bounds__(320, 1)
 kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs p) {
   using C = Cfg<KH, MT, NQ>;
-  constexpr int BKV = C::BKV, NS = C::NS, NO = C::NO, ST = C::STAGES;
+  constexpr int BKV = C::BKV, NS = C::NS, NO = C::NO, ST = C::STAGES, LA = C::LA;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* k_s = smem;
@@ -88,13 +93,11 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   uint8_t* q_s = v_s + ST * C::V_BYTES;
   uint8_t* p_s = q_s + C::Q_BYTES;                        // [2], each on 1024 bytes
   uint64_t* bars = reinterpret_cast<uint64_t*>(p_s + 2 * C::P_BYTES);
-  uint64_t* k_full = bars;         // [6]
-  uint64_t* k_empty = bars + 6;
+  uint64_t* k_full = bars;         // [6] one per stage
+  uint64_t* k_done = bars + 6;     // scores made: for the softmax, and the stage is free
   uint64_t* v_full = bars + 12;
-  uint64_t* v_empty = bars + 18;
-  uint64_t* s_full = bars + 24;    // [2]
-  uint64_t* p_ready = bars + 26;   // [2]
-  uint64_t* o_done = bars + 28;    // [2]
+  uint64_t* v_done = bars + 18;    // P V done: P may be written, O touched, and the stage is free
+  uint64_t* p_ready = bars + 24;   // [2] one per warpgroup
   uint64_t* q_full = bars + 30;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -133,15 +136,11 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_done[i], 1);
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_done[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 128);
-      mbar_init(&o_done[i], 1);
-    }
+    for (int i = 0; i < 2; ++i) mbar_init(&p_ready[i], 128);
     mbar_init(q_full, 256);
     *abort_flag = 0;
     mbar_fence_init();
@@ -154,7 +153,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const uint32_t tmem_S = tmem_base, tmem_O = tmem_base + 2 * NS;
+  const uint32_t tmem_S = tmem_base, tmem_O = tmem_base + LA * NS;
   const int* bt = p.s.table + b * p.s.ld_table;
   const int ppb = BKV / c.page;
 
@@ -173,7 +172,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       }
       const int st = i % ST;
       for (int kv = 0; ok && kv < 2; ++kv) {
-        uint64_t* empty = kv ? &v_empty[st] : &k_empty[st];
+        uint64_t* empty = kv ? &v_done[st] : &k_done[st];
         uint64_t* full = kv ? &v_full[st] : &k_full[st];
         if (i >= ST && !__all_sync(0xffffffffu, mbar_wait(empty, ((i / ST) - 1) & 1, abort_flag))) {
           if (lane == 0) { *abort_flag = 1; atomicCAS(p.s.status, 0, ST_TIMEOUT_EMPTY | SITE_DECODE_ATTN); }
@@ -206,20 +205,18 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!mbar_wait(&k_full[st], (i / ST) & 1, abort_flag)) return fail(ST_TIMEOUT_FULL);
         tc_fence_after();
         const uint64_t da = dk + uint32_t(st) * (C::K_BYTES / 16);
-        const uint32_t ts = tmem_S + (i & 1) * NS;
+        const uint32_t ts = tmem_S + (i % LA) * NS;
 #pragma unroll
         for (int h = 0; h < KH; ++h) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             umma_f8(ts, da + (h * (BKV * 8) + k * 2), dq + (h * (NS * 8) + k * 2), idesc_s, (h | k) ? 1u : 0u);
         }
-        umma_commit(&s_full[i & 1]);
-        umma_commit(&k_empty[st]);
+        umma_commit(&k_done[st]);
         return true;
       };
       bool ok = mbar_wait(q_full, 0, abort_flag) || fail(ST_TIMEOUT_FULL);
-      ok = ok && issue_s(0);
-      if (ok && n_tiles > 1) ok = issue_s(1);
+      for (int i = 0; ok && i < min(LA, n_tiles); ++i) ok = issue_s(i);
       for (int i = 0; ok && i < n_tiles; ++i) {
         const int w = i & 1, st = i % ST;
         if (!mbar_wait(&p_ready[w], (i >> 1) & 1, abort_flag)) { fail(ST_TIMEOUT_FLAG); break; }
@@ -233,16 +230,15 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           for (int k = 0; k < BKV / 32; ++k)
             umma_f8(to + mt * NO, da + (mt * (BKV * 8) + k * 256), db + k * 2, idesc_o, ((i >> 1) | k) ? 1u : 0u);
         }
-        umma_commit(&o_done[w]);
-        umma_commit(&v_empty[st]);
-        if (i + 2 < n_tiles && !issue_s(i + 2)) break;
+        umma_commit(&v_done[st]);
+        if (i + LA < n_tiles && !issue_s(i + LA)) break;      // into the buffer of tile i, which its softmax has read
       }
     }
   } else {
     // ------------------------------------------------------------------ softmax (warps 0..7)
     const int w = warp >> 2, wq = warp & 3, tl = wq * 32 + lane;
     const uint32_t lane_off = uint32_t(wq * 32) << 16;
-    const uint32_t my_S = tmem_S + w * NS + lane_off, my_O = tmem_O + w * MT * NO + lane_off;
+    const uint32_t my_S = tmem_S + lane_off, my_O = tmem_O + w * MT * NO + lane_off;
     const int bar_id = 1 + w;
     float* red = s_red + w * (NQ * 4);
     uint8_t* my_p = p_s + w * C::P_BYTES;
@@ -338,13 +334,13 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const int ev = kv8_log2(vs);
       const float add = float(ev), inv_v = __uint_as_float(uint32_t(127 - ev) << 23);     // |ev| <= 120
       if (i + 2 < n_tiles) scales(tile0 + i + 2, ks, vs);       // the next tile's, while this one is worked on
-      if (ok && !__all_sync(0xffffffffu, mbar_wait(&s_full[w], (i >> 1) & 1, abort_flag))) fail(ST_TIMEOUT_TMEM_FULL);
+      if (ok && !__all_sync(0xffffffffu, mbar_wait(&k_done[i % ST], (i / ST) & 1, abort_flag))) fail(ST_TIMEOUT_TMEM_FULL);
       uint32_t r[NS];
 #pragma unroll
       for (int q = 0; q < NS; ++q) r[q] = 0u;
       if (ok) {
         tc_fence_after();
-        tm_ld<NS>(my_S, r);
+        tm_ld<NS>(my_S + (i % LA) * NS, r);
         tmem_ld_wait();
       }
       const int key0 = (tile0 + i) * BKV, tok = key0 + tl;
@@ -366,7 +362,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 128, p;\n\t"
           "selp.u32 %0, 1, 0, q;\n\t}"
           : "=r"(any_over) : "r"(over ? 1u : 0u), "r"(bar_id) : "memory");
-      if (ok && n_mine >= 1 && !__all_sync(0xffffffffu, mbar_wait(&o_done[w], ((i - 2) >> 1) & 1, abort_flag)))
+      if (ok && n_mine >= 1 && !__all_sync(0xffffffffu, mbar_wait(&v_done[(i - 2) % ST], ((i - 2) / ST) & 1, abort_flag)))
         fail(ST_TIMEOUT_TMEM_EMPTY);
       if (any_over) {
         float alpha[NQ];
@@ -446,7 +442,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
     if (ok && n_mine >= 1) {
       const int last = w + 2 * (n_mine - 1);
-      if (!__all_sync(0xffffffffu, mbar_wait(&o_done[w], (last >> 1) & 1, abort_flag))) fail(ST_TIMEOUT_TMEM_FULL);
+      if (!__all_sync(0xffffffffu, mbar_wait(&v_done[last % ST], (last / ST) & 1, abort_flag))) fail(ST_TIMEOUT_TMEM_FULL);
     }
     // sums over the keys; the second warpgroup hands its results to the first through the (now idle) key stages
 #pragma unroll
