@@ -82,7 +82,7 @@ void kv8_append(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor
 
 void kv8_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& table,
                    const Tensor& ctx, const Tensor& cu, int64_t max_new, double scale, int64_t window, double softcap, const OptT& sink,
-                   int64_t per, int64_t n_splits, Tensor& out, const Tensor& status, const OptT& weights, int64_t observe, int64_t w_per,
+                   int64_t n_splits, Tensor& out, const Tensor& status, const OptT& weights, int64_t observe, int64_t w_per,
                    int64_t w_splits) {
   const char* who = "kv8_attention";
   const auto c = cache_of(k, v, ks, vs, who);
@@ -110,16 +110,18 @@ void kv8_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   one_device(q, {&k, &v, &ks, &vs, &table, &ctx, &cu, &out, &status}, who);
   c10::cuda::CUDAGuard guard(q.device());
   if (T == 0 || s.n == 0 || max_new == 0) return;
-  LB_ASK(per >= 1 && n_splits >= 1 && n_splits <= 128 && n_splits * c.Hkv <= 65535 && T * Hq < (int64_t(1) << 31), who, ": splits, rows");
+  LB_ASK(n_splits >= 1 && n_splits <= 255 && n_splits * c.Hkv <= 65535 && T * Hq < (int64_t(1) << 31), who, ": splits, rows");
   Tensor part;
-  if (n_splits > 1) part = at::empty({T * Hq * n_splits * (c.dv + 2)}, q.options().dtype(at::kFloat));
+  const int64_t nq = lb::kv8_decode_heads(int(Hq / c.Hkv)), meta = 4 * n_splits;
+  if (max_new == 1) part = at::empty({meta + 2 * n_splits * nq * (c.dv + 2)}, q.options().dtype(at::kFloat));
+  else if (n_splits > 1) part = at::empty({T * Hq * n_splits * (c.dv + 2)}, q.options().dtype(at::kFloat));
   Tensor lse;
   if (weights.has_value()) {
     lse = at::empty({T * Hq}, q.options().dtype(at::kFloat));
     a.lse = lse.data_ptr<float>();
   }
-  float* pp = n_splits > 1 ? part.data_ptr<float>() : nullptr;
-  const int rc = max_new == 1 ? lb::kv8_decode_launch(c, s, a, int(per), int(n_splits), pp, cur_stream())
+  float* pp = part.defined() ? part.data_ptr<float>() : nullptr;
+  const int rc = max_new == 1 ? lb::kv8_decode_launch(c, s, a, int(n_splits), pp + meta, reinterpret_cast<int*>(pp), cur_stream())
                               : lb::kv8_prompt_launch(c, s, a, int(n_splits), pp, cur_stream());
   TORCH_CHECK(rc == 0, "kv8_attention: ", lb::kv8_last_error());
   if (weights.has_value())

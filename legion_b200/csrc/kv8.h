@@ -1,4 +1,5 @@
-// Launch interface of the 8-bit key/value cache (kv8_cache.cu, attn_kv8_decode_sm100.cu). A cache is e4m3 codes
+// Launch interface of the 8-bit key/value cache (kv8_cache.cu, kv8_evict.cu, attn_kv8_decode_sm100.cu,
+// attn_kv8_prompt_sm100.cu, kv8_weights_sm100.cu). A cache is e4m3 codes
 // [blocks, kv heads, page, head size] for keys and for values and one float32 scale, a power of two, per block and head
 // [blocks, kv heads]; a value is its code times its block's scale. Pointers are device pointers; every function returns 0 on
 // success and enqueues without synchronising.
@@ -39,10 +40,12 @@ struct Kv8Attn {
   void* out; long o_tok;                // bf16 [T, Hq * dv], elements between rows
   float* lse;                           // [T, Hq] log2 of the sum of the exponentials, or nullptr
 };
-// Decode (max_new == 1): tiles of 128 keys, `per` of them to a split. part: splits of every row and head, dv + 2 floats each
-// (splits = ceil(ceil(max_ctx / 128) / per), 1 needs none).
-int kv8_decode_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int per, int n_splits, float* part, cudaStream_t st);
-// Prompts and rows behind a context: the tiles of 128 keys that a tile of rows sees fall into n_splits parts; part as above.
+// Decode (max_new == 1) on `ctas` CTAs, 255 at most. part: 2 * ctas * kv8_decode_heads(Hq / Hkv) * (dv + 2) floats, meta: 4 * ctas ints
+// on 16 bytes.
+int kv8_decode_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int ctas, float* part, int* meta, cudaStream_t st);
+int kv8_decode_heads(int group);
+// Prompts and rows behind a context: the tiles of 128 keys that a tile of rows sees fall into n_splits parts.
+// part: n_splits * (dv + 2) floats for every row and head, where n_splits > 1.
 int kv8_prompt_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int n_splits, float* part, cudaStream_t st);
 // Joins the partial results of every row and head of a prompt call.
 cudaError_t kv8_join(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int n_splits, float* part, cudaStream_t st);

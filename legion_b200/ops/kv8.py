@@ -75,14 +75,6 @@ def kv8_append(cache: Kv8Cache, k, v, block_table, ctx_lens, cu_q, max_q_len: in
 
 
 @functools.lru_cache(maxsize=4096)
-def _decode_split(n: int, kv_heads: int, group: int, tiles: int) -> Tuple[int, int]:
-    """(tiles of 128 keys to a split, splits) of a decode call."""
-    s = _sm.decode_splits(n, kv_heads, (group + 15) // 16, tiles * 128)
-    per = -(-tiles // s)
-    return per, -(-tiles // per)
-
-
-@functools.lru_cache(maxsize=4096)
 def _prompt_splits(n: int, kv_heads: int, rows: int, row_tile: int, tiles: int) -> int:
     """Parts of a prompt call's keys: as many as make the waves of CTAs times their tiles (and what a part costs beside them)
     least."""
@@ -134,13 +126,13 @@ def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: in
         tiles = min(tiles, -(-window // 128) + 1)
     group = q.shape[1] // k.shape[1]
     if max_q_len == 1:
-        per, splits = _decode_split(block_table.shape[0], k.shape[1], group, tiles)
+        splits = min(_sm.NUM_SMS, block_table.shape[0] * k.shape[1] * -(-group // (8 if group <= 8 else 16)) * tiles)      # CTAs
     else:
         rows = 256 if k.shape[3] <= 128 and cache.v.shape[3] <= 128 else 128
-        per, splits = 1, _prompt_splits(block_table.shape[0], k.shape[1], max_q_len * group, rows, tiles + max_q_len // 128)
+        splits = _prompt_splits(block_table.shape[0], k.shape[1], max_q_len * group, rows, tiles + max_q_len // 128)
     w_per, w_splits = (1, 1) if weights is None else _weight_split(block_table.shape[0], k.shape[1], max(1, -(-span // 128)))
     _sm.ext().kv8_attention(q, k, cache.v, cache.k_scale, cache.v_scale, block_table, ctx_lens, cu_q, max_q_len, scale, window,
-                            softcap, sink, per, splits, out, _sm.Workspace.get(q.device).status, weights, observe, w_per, w_splits)
+                            softcap, sink, splits, out, _sm.Workspace.get(q.device).status, weights, observe, w_per, w_splits)
     return out
 
 

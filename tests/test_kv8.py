@@ -375,6 +375,21 @@ def test_prompt_propagates_nan_to_rows_that_see_it(device):
 
 
 @pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("heads,kv,D,lens", [(8, 2, 64, [(37 * i) % 300 for i in range(150)]), (4, 4, 32, [1] * 300),
+                                             (34, 2, 64, [128, 129, 0, 640, 1, 1, 2000, 5])])
+def test_decode_batches(device, heads, kv, D, lens):
+    """Batches whose lengths are spread over the CTAs: more sequences than are kept at hand, groups inside and across CTAs, short
+    ones in a row, lengths of zero, rows that not every sequence has."""
+    cache, table = filled(lens, 16, kv, D, D, seed=11, device=device)
+    new = [0 if i % 13 == 5 else 1 for i in range(len(lens))]
+    q = randn(sum(new), heads, D, seed=12).bfloat16()
+    want, tol, _, _ = attend(q, cache, table, lens, new, 0.2)
+    got = ops.kv8_attention(q.to(device), cache, i32(table, device), i32(lens, device), i32(cum(new), device), 1, 0.2)
+    assert status(device) == 0
+    near(got, want, tol)
+
+
+@pytest.mark.parametrize("device", WHERE)
 def test_decode_rows_apart(device):
     """Queries cut out of a projection, an output with rows of its own pitch, sequences without a row, max_ctx."""
     lens, heads, kv, D = [200, 77, 300], 8, 2, 64
@@ -646,7 +661,7 @@ def test_refusals_need_no_gpu(what):
     C, st = ops.sm100.ext(), torch.zeros(4, dtype=torch.int32)
     out = torch.zeros(1, a["q"].shape[1], c.v.shape[3], dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="kv8_attention"):
-        C.kv8_attention(a["q"], c.k, c.v, c.k_scale, c.v_scale, a["table"], a["ctx"], a["cu"], 1, 0.1, kw["window"], kw["softcap"], None, 1, 1,
+        C.kv8_attention(a["q"], c.k, c.v, c.k_scale, c.v_scale, a["table"], a["ctx"], a["cu"], 1, 0.1, kw["window"], kw["softcap"], None, 1,
                         out, st, None, 0, 1, 1)
     if what in ("scale type", "int64 lengths", "bounds", "page", "code type", "devices"):
         with pytest.raises(ValueError, match="kv8_append"):
@@ -678,7 +693,7 @@ def test_refusals_of_sums_and_eviction_need_no_gpu(what):
         budget = 0
     if what in ("sums type", "sums shape", "rows overlap", "observe"):
         with pytest.raises(ValueError, match="kv8_attention"):
-            C.kv8_attention(a["q"], c.k, c.v, c.k_scale, c.v_scale, a["table"], a["ctx"], a["cu"], 1, 0.1, 0, 0.0, None, 1, 1,
+            C.kv8_attention(a["q"], c.k, c.v, c.k_scale, c.v_scale, a["table"], a["ctx"], a["cu"], 1, 0.1, 0, 0.0, None, 1,
                             torch.zeros(1, 4, 32, dtype=torch.bfloat16), st, w, observe, 1, 1)
     if what != "observe":
         with pytest.raises(ValueError, match="kv8_evict"):
