@@ -19,10 +19,11 @@
 // 64 sequences of 750 to 2250 tokens, 40 / 8 heads of 128, took 94 us.) Scratch belongs to the call.
 //
 // Two softmax warpgroups (warps 0..3 and 4..7; thread = key of the tile, later output column) take alternate tiles, each a
-// stream of its own with its P and O^T; they meet in shared memory at the end of a piece. Warp 8: MMAs, scores four tiles ahead
+// stream of its own with its P and O^T; they meet in shared memory at the end of a piece. Warp 8: the scores' MMAs, four tiles ahead
 // of their softmax (a wait for a phase of a stage's barrier cannot miss it: the stage's next scores stand behind P of this tile,
-// the stage's next P V behind P of the tile that waits). Warp 9: TMA through the block table into as many stages as 192 KB hold
-// (six of 32 KB for heads of 128), and the tiles' scales. Warps 10, 11: the next piece's queries.
+// the stage's next P V behind P of the tile that waits). Warp 9: TMA through the block table into as many stages as fit
+// (six of 32 KB for heads of 128), and the tiles' scales. Warp 10: the next piece's queries. Warp 11: P V. Code that runs
+// once a piece or rarely is kept short: unrolled over the heads it was fetched at 6000 clocks a piece.
 #include "kv8_dev.cuh"
 #include "tmap.cuh"
 
@@ -44,12 +45,6 @@ struct DecodeArgs {
 // quarter of the tiles of a stream of 2000 keys, 1900 clocks each.)
 constexpr float OFFSET = 11.f;
 constexpr float SLACK = 4.f;
-
-__device__ __forceinline__ int ordered(float f) {
-  const int i = __float_as_int(f);
-  return i >= 0 ? i : i ^ 0x7fffffff;
-}
-__device__ __forceinline__ float unordered(int i) { return __int_as_float(i >= 0 ? i : i ^ 0x7fffffff); }
 
 template <int N>
 __device__ __forceinline__ void tm_ld(uint32_t at, uint32_t* r) {
@@ -76,16 +71,21 @@ struct Cfg {
   static constexpr int BKV = 128;
   static constexpr int NS = 2 * NQ, NO = (3 * NQ + 15) / 16 * 16;
   static constexpr int K_BYTES = KH * BKV * 128, V_BYTES = MT * BKV * 128;
-  static constexpr int STAGES = 192 * 1024 / (K_BYTES + V_BYTES);          // 6, 4 or 3
-  static constexpr int Q_BYTES = KH * NS * 128, P_BYTES = NO * 128;        // two of each
+  static constexpr int Q_BYTES = KH * NS * 128, P_BYTES = NO * 128;
   static constexpr int SEQS = 128;                                         // lengths kept in shared memory
-  static constexpr int SC = 512 + 512 + 256, SEQ = SC + 16 * 16 * 8;       // offsets in the tail
+  static constexpr int SC = 1472, SEQ = SC + 16 * 16 * 8;       // offsets in the tail
   static constexpr int TAIL = SEQ + SEQS * 8;
-  static constexpr int SMEM = STAGES * (K_BYTES + V_BYTES) + 2 * Q_BYTES + 2 * P_BYTES + TAIL + 1024;
+  // P of a tile may be written while P V two tiles back still reads the other buffer, where four stages or more are left (with
+  // three, the wait for P V four tiles back could miss its phase)
+  static constexpr int ROOM = 227 * 1024 - TAIL - 1024 - 2 * Q_BYTES;
+  static constexpr int TWO = (ROOM - 4 * P_BYTES) / (K_BYTES + V_BYTES), ONE = (ROOM - 2 * P_BYTES) / (K_BYTES + V_BYTES);
+  static constexpr int PB = TWO >= 4 ? 2 : 1;                              // P buffers of a warpgroup
+  static constexpr int STAGES = PB == 2 ? (TWO > 6 ? 6 : TWO) : (ONE > 6 ? 6 : ONE);
+  static constexpr int SMEM = STAGES * (K_BYTES + V_BYTES) + 2 * Q_BYTES + 2 * PB * P_BYTES + TAIL + 1024;
   static constexpr int LA = STAGES < 4 ? STAGES : 4;                       // tiles whose scores are made ahead
   static constexpr int TMEM_RAW = LA * NS + 2 * MT * NO;
   static constexpr int TMEM_COLS = TMEM_RAW <= 128 ? 128 : TMEM_RAW <= 256 ? 256 : 512;
-  static_assert(TMEM_RAW <= 512 && STAGES >= 3 && STAGES <= 6 && SMEM <= 227 * 1024 && P_BYTES >= 8 * 128 * 4, "sizes");
+  static_assert(TMEM_RAW <= 512 && STAGES >= 3 && STAGES <= 6 && SMEM <= 227 * 1024 && (PB == 1 || STAGES >= 4) && P_BYTES >= 8 * 128 * 4, "sizes");
 };
 
 // A sequence's first tile, tiles (at least one if it has a row: a row that sees nothing is a result, too), length and row
@@ -129,30 +129,30 @@ template <int KH, int MT, int NQ, bool CAP>
 __global__ void __launch_bounds__(384, 1)
 kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs p) {
   using C = Cfg<KH, MT, NQ>;
-  constexpr int BKV = C::BKV, NS = C::NS, NO = C::NO, ST = C::STAGES, LA = C::LA;
+  constexpr int BKV = C::BKV, NS = C::NS, NO = C::NO, ST = C::STAGES, LA = C::LA, PB = C::PB;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* k_s = smem;
   uint8_t* v_s = k_s + ST * C::K_BYTES;
   uint8_t* q_s = v_s + ST * C::V_BYTES;                   // [2]
-  uint8_t* p_s = q_s + 2 * C::Q_BYTES;                    // [2], each on 1024 bytes
-  uint8_t* tail = p_s + 2 * C::P_BYTES;
+  uint8_t* p_s = q_s + 2 * C::Q_BYTES;                    // [2 warpgroups][PB], each on 1024 bytes
+  uint8_t* tail = p_s + 2 * PB * C::P_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(tail);
   uint64_t* k_full = bars;         // [6] one per stage
   uint64_t* k_done = bars + 6;     // scores made: for the softmax, and the stage is free
   uint64_t* v_full = bars + 12;
   uint64_t* v_done = bars + 18;    // P V done: P may be written, O touched, and the stage is free
-  uint64_t* p_ready = bars + 24;   // [2] one per warpgroup
-  uint64_t* q_free = bars + 26;    // [2] scores of a piece made
-  uint64_t* q_full = bars + 28;    // [8] a piece's queries and their power of two
-  uint64_t* sc_full = bars + 36;   // [16] a tile's scales
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 52);
+  uint64_t* p_ready = bars + 24;   // [4] tile % 4: a warpgroup may be through with a tile before P V of its last one is issued
+  uint64_t* q_free = bars + 28;    // [2] scores of a piece made
+  uint64_t* q_full = bars + 30;    // [8] a piece's queries and their power of two
+  uint64_t* sc_full = bars + 38;   // [16] a tile's scales
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 54);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* s_red = reinterpret_cast<float*>(tail + 512);    // [2 warpgroups][NQ][4 warps] maxima, then sums
-  float* ml_x = reinterpret_cast<float*>(tail + 1024);    // [NQ][2]
-  float* fq_s = reinterpret_cast<float*>(tail + 1152);    // [8]
-  uint32_t* s_qmax = reinterpret_cast<uint32_t*>(tail + 1184);   // [2]
-  int* s_start = reinterpret_cast<int*>(tail + 1200);     // sequence, group, tile, units, and the batch's units (64 bits)
+  float* s_ref = reinterpret_cast<float*>(tail + 1024);   // [2 warpgroups][references NQ, factors NQ]
+  float2* s_fac = reinterpret_cast<float2*>(tail + 1280); // [NQ] what each warpgroup's sums count in the result
+  float* fq_s = reinterpret_cast<float*>(tail + 1408);    // [8]
+  int* s_start = reinterpret_cast<int*>(tail + 1440);     // sequence, group, tile, units, and the batch's units (64 bits)
   float2* s_sc = reinterpret_cast<float2*>(tail + C::SC); // [16][16] scales of keys and values per 8 keys
   int2* s_seq = reinterpret_cast<int2*>(tail + C::SEQ);   // length, row (-1: none)
 
@@ -167,11 +167,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       mbar_init(&v_full[i], 1);
       mbar_init(&v_done[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&p_ready[i], 128);
-      mbar_init(&q_free[i], 1);
-    }
-    for (int i = 0; i < 8; ++i) mbar_init(&q_full[i], 64);
+    for (int i = 0; i < 4; ++i) mbar_init(&p_ready[i], 128);
+    for (int i = 0; i < 2; ++i) mbar_init(&q_free[i], 1);
+    for (int i = 0; i < 8; ++i) mbar_init(&q_full[i], 32);
     for (int i = 0; i < 16; ++i) mbar_init(&sc_full[i], 32);
     *abort_flag = 0;
     mbar_fence_init();
@@ -299,69 +297,71 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       }
     }
   } else if (warp == 8) {
-    // ------------------------------------------------------------------ MMA issuer
+    // ------------------------------------------------------------------ scores (one thread issues)
+    // Descriptors are made once; a step adds its offset in 16-byte units. (Made anew for every MMA they take the issuing thread
+    // 170 clocks each; an MMA of this shape takes 40.)
     if (lane == 0) {
-      constexpr uint32_t idesc_s = umma_idesc(128, NS, 0, 0, 0, 0);       // e4m3 x e4m3
-      constexpr uint32_t idesc_o = umma_idesc(128, NO, 0, 1, 1, 0);       // e4m3 (V^T, MN-major) x e5m2
-      // Descriptors are made once; a step adds its offset in 16-byte units. (Made anew for every MMA they take the one issuing
-      // thread 170 clocks each; an MMA of this shape takes 40.)
+      constexpr uint32_t idesc = umma_idesc(128, NS, 0, 0, 0, 0);         // e4m3 x e4m3
       const uint64_t dk = umma_desc_k_sw128(smem_u32(k_s)), dq = umma_desc_k_sw128(smem_u32(q_s));
-      const uint64_t dv = umma_desc_mn_sw128(smem_u32(v_s), BKV * 128, 1024), dp = umma_desc_k_sw128(smem_u32(p_s));
-      auto fail = [&](int code) { *abort_flag = 1; atomicCAS(p.s.status, 0, code | SITE_DECODE_ATTN); return false; };
-      Pieces<decltype(seq)> a(seq, groups, n_seqs, s_start[0], s_start[1], s_start[2], units);      // ahead: scores
-      int ja = 0, sa = 0, ia = 0;
-      auto issue_s = [&]() -> bool {
-        const int st = ia % ST;
-        if (ja == 0 && !mbar_wait(&q_full[sa & 7], (sa >> 3) & 1, abort_flag)) return fail(ST_TIMEOUT_FULL);
-        if (!mbar_wait(&k_full[st], (ia / ST) & 1, abort_flag)) return fail(ST_TIMEOUT_FULL);
-        tc_fence_after();
-        const uint64_t da = dk + uint32_t(st) * (C::K_BYTES / 16), db = dq + uint32_t(sa & 1) * (C::Q_BYTES / 16);
-        const uint32_t ts = tmem_S + (ia % LA) * NS;
-#pragma unroll
-        for (int h = 0; h < KH; ++h) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f8(ts, da + (h * (BKV * 8) + k * 2), db + (h * (NS * 8) + k * 2), idesc_s, (h | k) ? 1u : 0u);
-        }
-        umma_commit(&k_done[st]);
-        ++ia;
-        if (++ja == a.n()) {
-          umma_commit(&q_free[sa & 1]);
-          a.next();
-          ja = 0;
-          ++sa;
-        }
-        return true;
-      };
       bool ok = true;
-      for (int i = 0; ok && i < min(LA, units); ++i) ok = issue_s();
+      int i = 0, sn = 0;
+      for (Pieces<decltype(seq)> s(seq, groups, n_seqs, s_start[0], s_start[1], s_start[2], units); ok && s.left > 0; s.next(), ++sn) {
+        const int end = i + s.n();
+        ok = mbar_wait(&q_full[sn & 7], (sn >> 3) & 1, abort_flag);
+        const uint64_t db = dq + uint32_t(sn & 1) * (C::Q_BYTES / 16);
+        for (; ok && i < end; ++i) {
+          const int st = i % ST;
+          // into the buffer of tile i - LA, which its softmax has read
+          ok = (i < LA || mbar_wait(&p_ready[(i - LA) & 3], ((i - LA) >> 2) & 1, abort_flag)) && mbar_wait(&k_full[st], (i / ST) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t da = dk + uint32_t(st) * (C::K_BYTES / 16);
+          const uint32_t ts = tmem_S + (i % LA) * NS;
+#pragma unroll
+          for (int h = 0; h < KH; ++h) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_f8(ts, da + (h * (BKV * 8) + k * 2), db + (h * (NS * 8) + k * 2), idesc, (h | k) ? 1u : 0u);
+          }
+          umma_commit(&k_done[st]);
+        }
+        if (ok) umma_commit(&q_free[sn & 1]);
+      }
+      if (!ok) { *abort_flag = 1; atomicCAS(p.s.status, 0, ST_TIMEOUT_FULL | SITE_DECODE_ATTN); }
+    }
+  } else if (warp == 11) {
+    // ------------------------------------------------------------------ P V (one thread issues; beside the scores' thread: one
+    // thread for both took 1100 clocks a tile, four fifths of what its bytes take)
+    if (lane == 0) {
+      constexpr uint32_t idesc = umma_idesc(128, NO, 0, 1, 1, 0);         // e4m3 (V^T, MN-major) x e5m2
+      const uint64_t dv = umma_desc_mn_sw128(smem_u32(v_s), BKV * 128, 1024), dp = umma_desc_k_sw128(smem_u32(p_s));
+      bool ok = true;
       int i = 0;
       for (Pieces<decltype(seq)> s(seq, groups, n_seqs, s_start[0], s_start[1], s_start[2], units); ok && s.left > 0; s.next()) {
-        const int n = s.n();
-        for (int j = 0; ok && j < n; ++j, ++i) {
-          const int w = i & 1, st = i % ST;
-          if (!mbar_wait(&p_ready[w], (i >> 1) & 1, abort_flag)) { ok = fail(ST_TIMEOUT_FLAG); break; }
-          if (!mbar_wait(&v_full[st], (i / ST) & 1, abort_flag)) { ok = fail(ST_TIMEOUT_FULL); break; }
+        const int begin = i, end = i + s.n();
+        for (; ok && i < end; ++i) {
+          const int st = i % ST;
+          ok = mbar_wait(&p_ready[i & 3], (i >> 2) & 1, abort_flag) && mbar_wait(&v_full[st], (i / ST) & 1, abort_flag);
+          if (!ok) break;
           tc_fence_after();
-          const uint64_t da = dv + uint32_t(st) * (C::V_BYTES / 16), db = dp + uint32_t(w) * (C::P_BYTES / 16);
-          const uint32_t to = tmem_O + w * MT * NO;
+          const uint64_t da = dv + uint32_t(st) * (C::V_BYTES / 16), db = dp + uint32_t((i & 1) * PB + (i >> 1) % PB) * (C::P_BYTES / 16);
+          const uint32_t to = tmem_O + (i & 1) * MT * NO, more = i - begin >= 2;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
             for (int k = 0; k < BKV / 32; ++k)
-              umma_f8(to + mt * NO, da + (mt * (BKV * 8) + k * 256), db + k * 2, idesc_o, (j >= 2 || k) ? 1u : 0u);
+              umma_f8(to + mt * NO, da + (mt * (BKV * 8) + k * 256), db + k * 2, idesc, k ? 1u : more);
           }
           umma_commit(&v_done[st]);
-          if (ia < units) ok = issue_s();      // into the buffer of tile i, which its softmax has read
         }
       }
+      if (!ok) { *abort_flag = 1; atomicCAS(p.s.status, 0, ST_TIMEOUT_FLAG | SITE_DECODE_ATTN); }
     }
-  } else if (warp >= 10) {
+  } else if (warp == 10) {
     // ------------------------------------------------------------------ queries of the pieces
     // One power of two for all heads of a piece (what a smaller head loses is 2^-21 of the largest query value, and a softmax sees
     // absolute errors of its scores); a value that is not finite is a NaN code and makes its head NaN.
-    const int id = threadIdx.x - 320;
-    constexpr int CHUNKS = NQ * KH * 8, PER = CHUNKS / 64;              // of 16 values
+    constexpr int PER = NQ * KH / 4;                                    // chunks of 16 values of a lane
     int sn = 0;
     bool ok = true;
     for (Pieces<decltype(seq)> s(seq, groups, n_seqs, s_start[0], s_start[1], s_start[2], units); s.left > 0; s.next(), ++sn) {
@@ -370,7 +370,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       uint32_t m = 0;
 #pragma unroll
       for (int r = 0; r < PER; ++r) {
-        const int q = (id + r * 64) / (KH * 8), ch = (id + r * 64) % (KH * 8);
+        const int q = (lane + r * 32) / (KH * 8), ch = (lane + r * 32) % (KH * 8);
 #pragma unroll
         for (int i = 0; i < 8; ++i) u[r][i] = 0u;
         if (q < gn && ch * 16 < c.dk) {
@@ -394,10 +394,6 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
       }
       m = __reduce_max_sync(0xffffffffu, m);
-      if (lane == 0) s_qmax[warp - 10] = m;
-      named_sync<4, 64>();
-      m = max(s_qmax[0], s_qmax[1]);
-      named_sync<4, 64>();
       const float qs = kv8_scale_of(__uint_as_float(m << 16)), inv = kv8_inverse(qs);
       // the buffer held the queries of two pieces ago
       if (ok && sn >= 2 && !__all_sync(0xffffffffu, mbar_wait(&q_free[sn & 1], ((sn >> 1) - 1) & 1, abort_flag))) {
@@ -408,7 +404,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       uint8_t* qb = q_s + (sn & 1) * C::Q_BYTES;
 #pragma unroll
       for (int r = 0; r < PER; ++r) {
-        const int q = (id + r * 64) / (KH * 8), ch = (id + r * 64) % (KH * 8);
+        const int q = (lane + r * 32) / (KH * 8), ch = (lane + r * 32) % (KH * 8);
         uint32_t hi4[4], lo4[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -432,7 +428,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
       }
       // (eight slots: scores run at most four tiles, so four pieces ahead, queries two more)
-      if (id == 0) fq_s[sn & 7] = qs * (CAP ? p.cap_k : p.scale_log2);
+      if (lane == 0) fq_s[sn & 7] = qs * (CAP ? p.cap_k : p.scale_log2);
       fence_proxy_async_smem();
       mbar_arrive(&q_full[sn & 7]);
     }
@@ -443,8 +439,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const uint32_t my_S = tmem_S + lane_off, my_O = tmem_O + w * MT * NO + lane_off;
     const int bar_id = 1 + w;
     float* red = s_red + w * (NQ * 4);
-    uint8_t* my_p = p_s + w * C::P_BYTES;
-    float* x_s = reinterpret_cast<float*>(p_s + C::P_BYTES);      // the second warpgroup's P, idle at the end of a piece
+    float* s_m = s_ref + w * (2 * NQ);                           // references of the heads, and what O shrank by last
+    float* s_alpha = s_m + NQ;
+    float* x_s = reinterpret_cast<float*>(p_s + PB * C::P_BYTES);      // the second warpgroup's P, idle at the end of a piece
     // A wait that runs out does not leave the loops: the warp keeps taking part in the named barriers, without waiting again.
     bool ok = true;
     auto fail = [&](int code) { *abort_flag = 1; atomicCAS(p.s.status, 0, code | SITE_DECODE_ATTN); ok = false; };
@@ -458,6 +455,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       float m_ref[NQ], l_run[NQ];
 #pragma unroll
       for (int q = 0; q < NQ; ++q) { m_ref[q] = -INFINITY; l_run[q] = 0.f; }
+      if (tl < NQ) s_m[tl] = -INFINITY;        // (nobody reads the last piece's any more)
       int n_mine = 0;
       const int end = it + n;
       for (int i = it + ((it ^ w) & 1); i < end; i += 2, ++n_mine) {
@@ -494,32 +492,35 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 128, p;\n\t"
             "selp.u32 %0, 1, 0, q;\n\t}"
             : "=r"(any_over) : "r"(over ? 1u : 0u), "r"(bar_id) : "memory");
-        // this warpgroup's P V before (two tiles back) read P and wrote O
-        if (ok && n_mine >= 1 && !__all_sync(0xffffffffu, mbar_wait(&v_done[(i - 2) % ST], ((i - 2) / ST) & 1, abort_flag)))
+        // the P V that read this P buffer; where O moves, the one before
+        const int back = any_over || PB == 1 ? 2 : 4;
+        if (ok && n_mine >= back / 2 && !__all_sync(0xffffffffu, mbar_wait(&v_done[(i - back) % ST], ((i - back) / ST) & 1, abort_flag)))
           fail(ST_TIMEOUT_TMEM_EMPTY);
+        uint8_t* my_p = p_s + (w * PB + (i >> 1) % PB) * C::P_BYTES;
         if (any_over) {
-          float alpha[NQ];
+          // a thread per head finds its new reference, and what sums and O shrink by; everybody takes them from shared memory
 #pragma unroll
           for (int q = 0; q < NQ; ++q) {
-            if (q < gn) {
-              const int wm = __reduce_max_sync(0xffffffffu, ordered(z[q]));
-              if (lane == q) red[q * 4 + wq] = unordered(wm);
-            }
+            float wm;
+            asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(wm) : "f"(z[q]));
+            if (lane == q) red[q * 4 + wq] = wm;
           }
           asm volatile("bar.sync %0, 128;" ::"r"(bar_id) : "memory");
-#pragma unroll
-          for (int q = 0; q < NQ; ++q) {
-            alpha[q] = 1.f;
-            if (q < gn) {
-              const float4 m4 = *reinterpret_cast<const float4*>(&red[q * 4]);
-              const float m = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
-              if (m > m_ref[q]) {
-                alpha[q] = m_ref[q] == -INFINITY ? 0.f : ex2(m_ref[q] - m);
-                m_ref[q] = m;
-              }
-              l_run[q] *= alpha[q];
-            }
+          if (tl < NQ) {
+            const float4 m4 = *reinterpret_cast<const float4*>(&red[tl * 4]);
+            const float old = s_m[tl], m = fmaxf(fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w)), old);
+            s_alpha[tl] = old == -INFINITY ? 0.f : ex2(old - m);
+            s_m[tl] = m;
           }
+          asm volatile("bar.sync %0, 128;" ::"r"(bar_id) : "memory");
+          float alpha[NQ];
+#pragma unroll
+          for (int q = 0; q < NQ; q += 4) {
+            *reinterpret_cast<float4*>(alpha + q) = *reinterpret_cast<const float4*>(s_alpha + q);
+            *reinterpret_cast<float4*>(m_ref + q) = *reinterpret_cast<const float4*>(s_m + q);
+          }
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) l_run[q] *= alpha[q];
           if (ok && n_mine >= 1) {
             tc_fence_after();
 #pragma unroll 1
@@ -534,7 +535,6 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           }
-          asm volatile("bar.sync %0, 128;" ::"r"(bar_id) : "memory");      // red is read before it is written again
         }
         // P: [term * NQ + head][key], K-major rows of 128 bytes, 128-byte swizzle. (Rows of heads that do not exist are columns of O
         // that nobody reads.)
@@ -572,7 +572,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
         fence_proxy_async_smem();
         tc_fence_before();
-        mbar_arrive(&p_ready[w]);
+        mbar_arrive(&p_ready[i & 3]);
       }
       it = end;
       if (ok && n_mine >= 1) {
@@ -582,83 +582,81 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       // ---- end of a piece: sums over the keys, the second warpgroup hands its results to the first, eight heads at a time
       const bool whole = s.t == 0 && n == s.i.tiles;
       float* part = p.part + ((long(blockIdx.x) * 2 + (s.t == 0 ? 1 : 0)) * NQ) * (D + 2);
+      // (lanes trade halves of the heads until each holds one head's sum over its lanes)
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        float v = l_run[q];
+      for (int o = NQ / 2; o >= 1; o >>= 1) {
+        const bool up = lane & o;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == q) red[q * 4 + wq] = v;
+        for (int q = 0; q < o; ++q) {
+          const float keep = up ? l_run[q + o] : l_run[q], give = up ? l_run[q] : l_run[q + o];
+          l_run[q] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
       }
-      asm volatile("bar.sync %0, 128;" ::"r"(bar_id) : "memory");
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        const float4 s4 = *reinterpret_cast<const float4*>(&red[q * 4]);
-        l_run[q] = (s4.x + s4.y) + (s4.z + s4.w);
-      }
-      if (w == 1 && tl == 0) {
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) { ml_x[2 * q] = m_ref[q]; ml_x[2 * q + 1] = l_run[q]; }
+      for (int o = NQ; o < 32; o <<= 1) l_run[0] += __shfl_xor_sync(0xffffffffu, l_run[0], o);
+      if (lane < NQ) red[lane * 4 + wq] = l_run[0];
+      named_sync<3, 256>();
+      if (threadIdx.x < NQ) {
+        const int q = threadIdx.x;
+        const float4 a4 = *reinterpret_cast<const float4*>(&s_red[q * 4]), b4 = *reinterpret_cast<const float4*>(&s_red[(NQ + q) * 4]);
+        const float l0 = (a4.x + a4.y) + (a4.z + a4.w), l1 = (b4.x + b4.y) + (b4.z + b4.w);
+        const float m0 = s_ref[q], m1 = s_ref[2 * NQ + q], m = fmaxf(m0, m1);
+        float f0 = m0 == -INFINITY ? (l0 == l0 ? 0.f : 1.f) : ex2(m0 - m);      // (NaN passes)
+        float f1 = m1 == -INFINITY ? (l1 == l1 ? 0.f : 1.f) : ex2(m1 - m);
+        float den = l0 * f0 + l1 * f1, top = m == -INFINITY ? m : m - OFFSET;
+        if (q < gn && whole) {
+          if (p.a.sink) {
+            const float sk = p.a.sink[head0 + q] * 1.4426950408889634f;
+            if (top == -INFINITY && den == 0.f) { top = sk; den = 1.f; }
+            else den += ex2(sk - top);
+          }
+          const float inv = den > 0.f || den != den ? 1.f / den : 0.f;
+          f0 *= inv;
+          f1 *= inv;
+          if (p.a.lse) p.a.lse[long(row) * p.a.Hq + head0 + q] = den > 0.f ? top + log2f(den) : -INFINITY;
+        } else if (q < gn) {
+          part[q * (D + 2) + D] = top;
+          part[q * (D + 2) + D + 1] = den;
+        }
+        s_fac[q] = make_float2(f0, f1);
       }
       tc_fence_after();
 #pragma unroll 1
       for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll 1
+        for (int h0 = 0; h0 < gn; h0 += 8) {
+          uint32_t o[3][8];
 #pragma unroll
-        for (int h0 = 0; h0 < NQ; h0 += 8) {
-          float acc[8];
-          {
-            uint32_t o[3][8];
+          for (int t = 0; t < 3; ++t) {
 #pragma unroll
-            for (int t = 0; t < 3; ++t) {
+            for (int j = 0; j < 8; ++j) o[t][j] = 0u;
+          }
+          if (ok && n_mine >= 1) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j) o[t][j] = 0u;
-            }
-            if (ok && n_mine >= 1) {
-#pragma unroll
-              for (int t = 0; t < 3; ++t)
-                asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                             : "=r"(o[t][0]), "=r"(o[t][1]), "=r"(o[t][2]), "=r"(o[t][3]), "=r"(o[t][4]), "=r"(o[t][5]), "=r"(o[t][6]),
-                               "=r"(o[t][7])
-                             : "r"(my_O + mt * NO + t * NQ + h0) : "memory");
-              tmem_ld_wait();
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] = __uint_as_float(o[0][j]) + (__uint_as_float(o[1][j]) + __uint_as_float(o[2][j]));
+            for (int t = 0; t < 3; ++t)
+              asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                           : "=r"(o[t][0]), "=r"(o[t][1]), "=r"(o[t][2]), "=r"(o[t][3]), "=r"(o[t][4]), "=r"(o[t][5]), "=r"(o[t][6]),
+                             "=r"(o[t][7])
+                           : "r"(my_O + mt * NO + t * NQ + h0) : "memory");
+            tmem_ld_wait();
           }
           if (w == 1) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x_s[j * 128 + tl] = acc[j];
+            for (int j = 0; j < 8; ++j)
+              x_s[j * 128 + tl] = __uint_as_float(o[0][j]) + (__uint_as_float(o[1][j]) + __uint_as_float(o[2][j]));
           }
           named_sync<3, 256>();
-          if (w == 0 && !*abort_flag) {
-            const int d = mt * 128 + tl;
+          const int d = mt * 128 + tl;
+          if (w == 0 && d < D && !*abort_flag) {
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.a.out) + row * p.a.o_tok + (head0 + h0) * D + d;
+            float* pd = part + h0 * (D + 2) + d;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const int q = h0 + j;
-              if (q < gn) {
-                const float m1 = ml_x[2 * q], l1 = ml_x[2 * q + 1];
-                const float m = fmaxf(m_ref[q], m1);
-                const float f0 = m_ref[q] == -INFINITY ? (l_run[q] == l_run[q] ? 0.f : 1.f) : ex2(m_ref[q] - m);      // (NaN passes)
-                const float f1 = m1 == -INFINITY ? (l1 == l1 ? 0.f : 1.f) : ex2(m1 - m);
-                const float ll = l_run[q] * f0 + l1 * f1;
-                const float ref = m == -INFINITY ? m : m - OFFSET;
-                const float o = acc[j] * f0 + x_s[j * 128 + tl] * f1;
-                if (whole) {
-                  float den = ll, top = ref;
-                  if (p.a.sink) {
-                    const float sk = p.a.sink[head0 + q] * 1.4426950408889634f;
-                    if (top == -INFINITY && den == 0.f) { top = sk; den = 1.f; }
-                    else den += ex2(sk - top);
-                  }
-                  const float inv = den > 0.f || den != den ? 1.f / den : 0.f;
-                  if (p.a.lse && d == 0) p.a.lse[long(row) * p.a.Hq + head0 + q] = den > 0.f ? top + log2f(den) : -INFINITY;
-                  if (d < D) static_cast<__nv_bfloat16*>(p.a.out)[row * p.a.o_tok + (head0 + q) * D + d] = __float2bfloat16(o * inv);
-                } else {
-                  if (d < D) part[q * (D + 2) + d] = o;
-                  if (d == 0) {
-                    part[q * (D + 2) + D] = ref;
-                    part[q * (D + 2) + D + 1] = ll;
-                  }
-                }
+              const float2 f = s_fac[h0 + j];
+              const float v = (__uint_as_float(o[0][j]) + (__uint_as_float(o[1][j]) + __uint_as_float(o[2][j]))) * f.x + x_s[j * 128 + tl] * f.y;
+              if (h0 + j < gn) {
+                if (whole) dst[j * D] = __float2bfloat16(v);
+                else pd[j * (D + 2)] = v;
               }
             }
           }
