@@ -21,8 +21,8 @@
 // Two softmax warpgroups (warps 0..3 and 4..7; thread = key of the tile, later output column) take alternate tiles, each a
 // stream of its own with its P and O^T; they meet in shared memory at the end of a piece. Warp 8: the scores' MMAs, four tiles ahead
 // of their softmax (a wait for a phase of a stage's barrier cannot miss it: the stage's next scores stand behind P of this tile,
-// the stage's next P V behind P of the tile that waits). Warp 9: TMA through the block table into as many stages as fit
-// (six of 32 KB for heads of 128), and the tiles' scales. Warp 10: the next piece's queries. Warp 11: P V. Code that runs
+// the stage's next P V behind P of the tile that waits). Warps 9, 12: TMA of keys and of values through the block
+// table into as many stages as fit (six of 32 KB for heads of 128), and the tiles' scales. Warp 10: the next piece's queries. Warp 11: P V. Code that runs
 // once a piece or rarely is kept short: unrolled over the heads it was fetched at 6000 clocks a piece.
 #include "kv8_dev.cuh"
 #include "tmap.cuh"
@@ -126,7 +126,7 @@ struct Pieces {
 };
 
 template <int KH, int MT, int NQ, bool CAP>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(416, 1)
 kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs p) {
   using C = Cfg<KH, MT, NQ>;
   constexpr int BKV = C::BKV, NS = C::NS, NO = C::NO, ST = C::STAGES, LA = C::LA, PB = C::PB;
@@ -153,7 +153,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   float2* s_fac = reinterpret_cast<float2*>(tail + 1280); // [NQ] what each warpgroup's sums count in the result
   float* fq_s = reinterpret_cast<float*>(tail + 1408);    // [8]
   int* s_start = reinterpret_cast<int*>(tail + 1440);     // sequence, group, tile, units, and the batch's units (64 bits)
-  float2* s_sc = reinterpret_cast<float2*>(tail + C::SC); // [16][16] scales of keys and values per 8 keys
+  float* s_sc = reinterpret_cast<float*>(tail + C::SC);   // [16][keys, values][16] a tile's scales per 8 keys
   int2* s_seq = reinterpret_cast<int2*>(tail + C::SEQ);   // length, row (-1: none)
 
   const Kv8Cache& c = p.c;
@@ -170,7 +170,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     for (int i = 0; i < 4; ++i) mbar_init(&p_ready[i], 128);
     for (int i = 0; i < 2; ++i) mbar_init(&q_free[i], 1);
     for (int i = 0; i < 8; ++i) mbar_init(&q_full[i], 32);
-    for (int i = 0; i < 16; ++i) mbar_init(&sc_full[i], 32);
+    for (int i = 0; i < 16; ++i) mbar_init(&sc_full[i], 64);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -242,57 +242,76 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   if (units <= 0 && threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
 
   if (units <= 0) {
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------ TMA: the lanes fetch table and scales, lane 0 issues
-    const int tiles_per_fill = 32 / ppb;
+  } else if (warp == 9 || warp == 12) {
+    // ------------------------------------------------------------------ TMA, keys (warp 9) and values (warp 12): the lanes hold
+    // the rows of the next 32 pages and their scales, lane 0 issues. Table entries and scales are fetched a fill ahead, into the
+    // next piece too. (One warp for both issued a tile in 2000 clocks.)
+    const bool val = warp == 12;
+    const CUtensorMap* tm = val ? &tmV : &tmK;
+    uint64_t* full = val ? v_full : k_full;
+    uint64_t* done = val ? v_done : k_done;
+    const float* scales = val ? c.v_scale : c.k_scale;
+    const int parts = val ? MT : KH, bytes = val ? C::V_BYTES : C::K_BYTES;
+    uint8_t* ring = val ? v_s : k_s;
+    const int fill = 32 / ppb;                             // tiles
+    using P = Pieces<decltype(seq)>;
+    P s(seq, groups, n_seqs, s_start[0], s_start[1], s_start[2], units);
+    // (block, head) of this lane's page of the tiles from j on; -1 behind the sequence
+    auto unit_of = [&](const P& x, int j) -> long {
+      const long page = long(x.i.tile0 + x.t + j) * ppb + lane;
+      if (page * c.page >= x.i.ctx || j * ppb + lane >= x.n() * ppb) return -1;
+      const int blk = p.s.table[x.b * p.s.ld_table + page];
+      if (unsigned(blk) >= unsigned(c.n_blocks)) {
+        atomicCAS(p.s.status, 0, ST_BAD_ARGS);
+        return -1;
+      }
+      return long(blk) * c.Hkv + x.hg / gtiles;
+    };
+    long next = unit_of(s, 0);
+    float next_sc = next >= 0 ? scales[next] : 0.f;
     bool ok = true;
-    int it = 0;
-    for (Pieces<decltype(seq)> s(seq, groups, n_seqs, s_start[0], s_start[1], s_start[2], units); ok && s.left > 0; s.next()) {
-      const int* bt = p.s.table + s.b * p.s.ld_table;
-      const int kvh = s.hg / gtiles, tile0 = s.i.tile0 + s.t, n = s.n(), ctx = s.i.ctx;
-      int pg_reg = 0;
-      float2 sc_reg = make_float2(0.f, 0.f);
+    int it = 0, st = 0, lap = 0;
+    for (; ok && s.left > 0; s.next()) {
+      const int n = s.n();
+      int row = 0;
+      float sc = 0.f;
       for (int j = 0; ok && j < n; ++j, ++it) {
-        const int slot = j % tiles_per_fill;
+        const int slot = j % fill;
         if (slot == 0) {
-          const long page = long(tile0 + j) * ppb + lane;
-          // pages behind the sequence: a block outside the cache, whose rows TMA fills with zeros
-          pg_reg = page * c.page < ctx ? bt[page] : c.n_blocks;
-          sc_reg = make_float2(0.f, 0.f);
-          if (unsigned(pg_reg) < unsigned(c.n_blocks)) {
-            const long u = long(pg_reg) * c.Hkv + kvh;
-            sc_reg = make_float2(c.k_scale[u], c.v_scale[u]);
-          } else {
-            if (page * c.page < ctx && lane < n * ppb) atomicCAS(p.s.status, 0, ST_BAD_ARGS);
-            pg_reg = c.n_blocks;
+          // a page behind the sequence, or a block outside the cache: rows that TMA fills with zeros
+          row = int(next >= 0 ? next : long(c.n_blocks) * c.Hkv) * c.page;
+          sc = next_sc;
+          if (j + fill < n) {
+            next = unit_of(s, j + fill);
+          } else if (s.left > n) {
+            P x = s;
+            x.next();
+            next = unit_of(x, 0);
           }
         }
-        const int st = it % ST;
-        for (int kv = 0; ok && kv < 2; ++kv) {
-          uint64_t* empty = kv ? &v_done[st] : &k_done[st];
-          uint64_t* full = kv ? &v_full[st] : &k_full[st];
-          if (it >= ST && !__all_sync(0xffffffffu, mbar_wait(empty, ((it / ST) - 1) & 1, abort_flag))) {
-            if (lane == 0) { *abort_flag = 1; atomicCAS(p.s.status, 0, ST_TIMEOUT_EMPTY | SITE_DECODE_ATTN); }
-            ok = false;
-            break;
+        if (it >= ST && !__all_sync(0xffffffffu, mbar_wait(&done[st], (lap - 1) & 1, abort_flag))) {
+          if (lane == 0) { *abort_flag = 1; atomicCAS(p.s.status, 0, ST_TIMEOUT_EMPTY | SITE_DECODE_ATTN); }
+          ok = false;
+          break;
+        }
+        uint8_t* dst = ring + st * bytes;
+        if (lane == 0) mbar_expect_tx(&full[st], bytes);
+        for (int g = 0; g < ppb; ++g) {
+          const int r = __shfl_sync(0xffffffffu, row, slot * ppb + g);
+          if (lane == 0) {
+            tma_load_2d(dst + g * c.page * 128, tm, &full[st], 0, r);
+            if (parts == 2) tma_load_2d(dst + BKV * 128 + g * c.page * 128, tm, &full[st], 128, r);
           }
-          uint8_t* dst = kv ? v_s + st * C::V_BYTES : k_s + st * C::K_BYTES;
-          if (lane == 0) mbar_expect_tx(full, kv ? C::V_BYTES : C::K_BYTES);
-          for (int g = 0; g < ppb; ++g) {
-            const int pg = __shfl_sync(0xffffffffu, pg_reg, slot * ppb + g);
-            if (lane == 0) {
-              for (int h = 0; h < (kv ? MT : KH); ++h)
-                tma_load_2d(dst + h * (BKV * 128) + g * c.page * 128, kv ? &tmV : &tmK, full, h * 128, (pg * c.Hkv + kvh) * c.page);
-            }
-          }
-          if (kv == 0) {
-            // slot it % 16 held tile it - 16, whose softmax is over: this key stage is free, so scores ST tiles back are made, and
-            // they stand behind P of the tile LA <= 4 before
-            const int g = slot * ppb + (lane & 15) * 8 / c.page;
-            const float a = __shfl_sync(0xffffffffu, sc_reg.x, g), b = __shfl_sync(0xffffffffu, sc_reg.y, g);
-            if (lane < 16) s_sc[(it & 15) * 16 + lane] = make_float2(a, b);
-            mbar_arrive(&sc_full[it & 15]);
-          }
+        }
+        // slot it % 16 held tile it - 16, whose softmax is over: this stage is free, so scores (and P V) ST tiles back are made, and
+        // scores stand behind P of the tile LA <= 4 before
+        const float a = __shfl_sync(0xffffffffu, sc, slot * ppb + (lane & 15) * 8 / c.page);
+        if (lane < 16) s_sc[((it & 15) * 2 + (val ? 1 : 0)) * 16 + lane] = a;
+        mbar_arrive(&sc_full[it & 15]);
+        if (slot == 1 || j + 1 == n || fill == 1) next_sc = next >= 0 ? scales[next] : 0.f;
+        if (++st == ST) {
+          st = 0;
+          ++lap;
         }
       }
     }
@@ -460,9 +479,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const int end = it + n;
       for (int i = it + ((it ^ w) & 1); i < end; i += 2, ++n_mine) {
         if (ok && !__all_sync(0xffffffffu, mbar_wait(&sc_full[i & 15], (i >> 4) & 1, abort_flag))) fail(ST_TIMEOUT_FULL);
-        const float2 sc = s_sc[(i & 15) * 16 + (tl >> 3)];
-        const float mul = fq * sc.x;
-        const int ev = kv8_log2(sc.y);
+        const float mul = fq * s_sc[(i & 15) * 32 + (tl >> 3)];
+        const int ev = kv8_log2(s_sc[(i & 15) * 32 + 16 + (tl >> 3)]);
         const float add = float(ev), inv_v = __uint_as_float(uint32_t(127 - ev) << 23);     // |ev| <= 120
         if (ok && !__all_sync(0xffffffffu, mbar_wait(&k_done[i % ST], (i / ST) & 1, abort_flag))) fail(ST_TIMEOUT_TMEM_FULL);
         uint32_t r[NS];
@@ -744,7 +762,7 @@ cudaError_t launch(const CUtensorMap* tk, const CUtensorMap* tv, const DecodeArg
   static DeviceOnce once;
   const cudaError_t e = once.shared_memory(reinterpret_cast<const void*>(kfn), smem);
   if (e != cudaSuccess) return e;
-  return launch_pdl(kfn, dim3(ctas), dim3(384), smem, st, *tk, *tv, p);
+  return launch_pdl(kfn, dim3(ctas), dim3(416), smem, st, *tk, *tv, p);
 }
 
 }  // namespace
