@@ -493,6 +493,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
         const int key0 = (tile0 + i - it) * BKV, tok = key0 + tl;
         const bool valid = tok >= start && tok < ctx;
+        const int rel = tok - s.i.tile0 * BKV;
+        float* sc_out = p.a.scores && rel < p.a.span ? p.a.scores + (long(row) * p.a.Hq + head0) * p.a.span + rel : nullptr;
         float z[NQ];
         bool over = false;
 #pragma unroll
@@ -501,6 +503,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           if (q < gn) {
             float x = fmaf(__uint_as_float(r[NQ + q]), 0.0625f, __uint_as_float(r[q])) * mul;
             if constexpr (CAP) x = fmaf(softcap_r(x, 1.f), p.scale_log2, 0.5f * p.scale_log2);
+            if (sc_out && valid) sc_out[q * long(p.a.span)] = x;
             if (valid) z[q] = x + add;
             over |= z[q] > m_ref[q] + SLACK;
           }

@@ -82,8 +82,7 @@ void kv8_append(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor
 
 void kv8_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& table,
                    const Tensor& ctx, const Tensor& cu, int64_t max_new, double scale, int64_t window, double softcap, const OptT& sink,
-                   int64_t n_splits, Tensor& out, const Tensor& status, const OptT& weights, int64_t observe, int64_t w_per,
-                   int64_t w_splits) {
+                   int64_t n_splits, Tensor& out, const Tensor& status, const OptT& weights, int64_t observe, int64_t tiles) {
   const char* who = "kv8_attention";
   const auto c = cache_of(k, v, ks, vs, who);
   LB_ASK(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.stride(2) == 1 && q.size(2) == c.dk, who,
@@ -95,7 +94,7 @@ void kv8_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   LB_ASK(out.scalar_type() == at::kBFloat16 && out.dim() == 3 && out.size(0) == T && out.size(1) == Hq && out.size(2) == c.dv &&
              out.stride(2) == 1 && (out.stride(1) == c.dv || Hq == 1), who, ": out is bfloat16 [rows, heads, value head size]");
   lb::Kv8Attn a{q.data_ptr(), long(q.stride(0)), long(q.stride(1)), int(Hq), float(scale), float(softcap), int(window), nullptr,
-                out.data_ptr(), long(out.stride(0)), nullptr};
+                out.data_ptr(), long(out.stride(0)), nullptr, nullptr, 0};
   if (sink.has_value()) {
     LB_ASK(sink->scalar_type() == at::kFloat && sink->is_contiguous() && sink->numel() == Hq && sink->device() == q.device(), who,
            ": sinks are float32 [heads]");
@@ -104,7 +103,7 @@ void kv8_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   const auto s = seqs_of(table, ctx, cu, max_new, T, status, who);
   if (weights.has_value()) {
     check_sums(*weights, s.n, c.Hkv, who);
-    LB_ASK(weights->device() == q.device() && observe >= 0 && observe < (int64_t(1) << 31) && w_per >= 1 && w_splits >= 1 && w_splits <= 65535,
+    LB_ASK(weights->device() == q.device() && observe >= 0 && observe < (int64_t(1) << 31) && tiles >= 1 && tiles <= (int64_t(1) << 23),
            who, ": sums of weights on the queries' device, observed rows not negative");
   }
   one_device(q, {&k, &v, &ks, &vs, &table, &ctx, &cu, &out, &status}, who);
@@ -115,19 +114,29 @@ void kv8_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   const int64_t nq = lb::kv8_decode_heads(int(Hq / c.Hkv)), meta = 4 * n_splits;
   if (max_new == 1) part = at::empty({meta + 2 * n_splits * nq * (c.dv + 2)}, q.options().dtype(at::kFloat));
   else if (n_splits > 1) part = at::empty({T * Hq * n_splits * (c.dv + 2)}, q.options().dtype(at::kFloat));
-  Tensor lse;
+  Tensor lse, scratch;
   if (weights.has_value()) {
     lse = at::empty({T * Hq}, q.options().dtype(at::kFloat));
     a.lse = lse.data_ptr<float>();
+    if (max_new == 1) {
+      scratch = at::empty({T * Hq * tiles * 128}, q.options().dtype(at::kFloat));
+      a.scores = scratch.data_ptr<float>();
+      a.span = int(tiles * 128);
+    } else {
+      scratch = at::empty({lb::kv8_weights_scratch(c, s, a, int(observe))}, q.options().dtype(at::kByte));
+    }
   }
   float* pp = part.defined() ? part.data_ptr<float>() : nullptr;
   const int rc = max_new == 1 ? lb::kv8_decode_launch(c, s, a, int(n_splits), pp + meta, reinterpret_cast<int*>(pp), cur_stream())
                               : lb::kv8_prompt_launch(c, s, a, int(n_splits), pp, cur_stream());
   TORCH_CHECK(rc == 0, "kv8_attention: ", lb::kv8_last_error());
-  if (weights.has_value())
-    TORCH_CHECK(lb::kv8_weights_launch(c, s, a, int(observe), int(w_per), int(w_splits), weights->data_ptr<float>(), long(weights->stride(0)),
-                                       long(weights->stride(1)), int(weights->size(2)), cur_stream()) == 0,
-                "kv8_attention: ", lb::kv8_last_error());
+  if (!weights.has_value()) return;
+  float* w = weights->data_ptr<float>();
+  const long ws = long(weights->stride(0)), wh = long(weights->stride(1));
+  const int keys = int(weights->size(2));
+  const int wc = max_new == 1 ? lb::kv8_score_sums_launch(c, s, a, a.scores, a.span, w, ws, wh, keys, cur_stream())
+                              : lb::kv8_weights_launch(c, s, a, int(observe), int(tiles), scratch.data_ptr(), w, ws, wh, keys, cur_stream());
+  TORCH_CHECK(wc == 0, "kv8_attention: ", lb::kv8_last_error());
 }
 
 void kv8_evict(const Tensor& k, const Tensor& v, const Tensor& ks, const Tensor& vs, const Tensor& table, const Tensor& ctx,

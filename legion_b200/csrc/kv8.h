@@ -39,6 +39,7 @@ struct Kv8Attn {
   const float* sink;                    // [Hq] or nullptr
   void* out; long o_tok;                // bf16 [T, Hq * dv], elements between rows
   float* lse;                           // [T, Hq] log2 of the sum of the exponentials, or nullptr
+  float* scores; int span;              // decode: [T, Hq, span] takes the scores (log2) from the first visible tile on, or nullptr
 };
 // Decode (max_new == 1) on `ctas` CTAs, 255 at most. part: 2 * ctas * kv8_decode_heads(Hq / Hkv) * (dv + 2) floats, meta: 4 * ctas ints
 // on 16 bytes.
@@ -49,10 +50,14 @@ int kv8_decode_heads(int group);
 int kv8_prompt_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int n_splits, float* part, cudaStream_t st);
 // Joins the partial results of every row and head of a prompt call.
 cudaError_t kv8_join(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int n_splits, float* part, cudaStream_t st);
-// w[sequence, kv head, key] += softmax weights of the sequence's last `observe` rows (0: all), with a.lse from the attention; key
-// tiles in n_splits CTAs of `per`.
-int kv8_weights_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int observe, int per, int n_splits, float* w, long w_seq,
+// w[sequence, kv head, key] += softmax weights of the sequence's last `observe` rows (0: all), with a.lse from the attention. Rows of
+// prompts: the longest context has `tiles` tiles of 128 keys at most; scratch of kv8_weights_scratch bytes, on 16 bytes. Decode: from
+// the scores that the attention left in a.scores.
+int kv8_weights_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int observe, int tiles, void* scratch, float* w, long w_seq,
                        long w_head, int w_keys, cudaStream_t st);
+int64_t kv8_weights_scratch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int observe);
+int kv8_score_sums_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, const float* scores, int span, float* w, long w_seq,
+                          long w_head, int w_keys, cudaStream_t st);
 
 // Eviction: of every sequence and kv head the first `first` tokens, the last `last` and those of the largest weights stay, `budget`
 // in all, in order, in the blocks of dst. s.cu and s.max_new are not used.

@@ -87,14 +87,6 @@ def _prompt_splits(n: int, kv_heads: int, rows: int, row_tile: int, tiles: int) 
     return best
 
 
-@functools.lru_cache(maxsize=4096)
-def _weight_split(n: int, kv_heads: int, tiles: int) -> Tuple[int, int]:
-    """(key tiles of a CTA, CTAs of a sequence and head) for the sums of weights: two CTAs an SM."""
-    s = max(1, min(tiles, -(-4 * _sm.NUM_SMS // (n * kv_heads))))
-    per = -(-tiles // s)
-    return per, -(-tiles // per)
-
-
 def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: int, scale: float, window: int = 0, softcap: float = 0.0,
                   sink=None, weights=None, observe: int = 0, max_ctx: Optional[int] = None, out=None):
     """Causal attention of the query rows ``q`` [T, heads, dk] over the cache; returns [T, heads, dv] (``out`` takes it; its rows
@@ -122,17 +114,16 @@ def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: in
         out = torch.empty(q.shape[0], q.shape[1], cache.v.shape[3], dtype=q.dtype, device=q.device)
     span = min(max_ctx or 1 << 30, block_table.shape[1] * k.shape[2])
     tiles = max(1, -(-span // 128))
-    if window > 0:
+    if window > 0 and max_q_len == 1:
         tiles = min(tiles, -(-window // 128) + 1)
     group = q.shape[1] // k.shape[1]
     if max_q_len == 1:
         splits = min(_sm.NUM_SMS, block_table.shape[0] * k.shape[1] * -(-group // (8 if group <= 8 else 16)) * tiles)      # CTAs
     else:
         rows = 256 if k.shape[3] <= 128 and cache.v.shape[3] <= 128 else 128
-        splits = _prompt_splits(block_table.shape[0], k.shape[1], max_q_len * group, rows, tiles + max_q_len // 128)
-    w_per, w_splits = (1, 1) if weights is None else _weight_split(block_table.shape[0], k.shape[1], max(1, -(-span // 128)))
+        splits = _prompt_splits(block_table.shape[0], k.shape[1], max_q_len * group, rows, tiles if window <= 0 else min(tiles, (window + max_q_len) // 128 + 1))
     _sm.ext().kv8_attention(q, k, cache.v, cache.k_scale, cache.v_scale, block_table, ctx_lens, cu_q, max_q_len, scale, window,
-                            softcap, sink, splits, out, _sm.Workspace.get(q.device).status, weights, observe, w_per, w_splits)
+                            softcap, sink, splits, out, _sm.Workspace.get(q.device).status, weights, observe, tiles)
     return out
 
 

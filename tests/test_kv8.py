@@ -662,7 +662,7 @@ def test_refusals_need_no_gpu(what):
     out = torch.zeros(1, a["q"].shape[1], c.v.shape[3], dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="kv8_attention"):
         C.kv8_attention(a["q"], c.k, c.v, c.k_scale, c.v_scale, a["table"], a["ctx"], a["cu"], 1, 0.1, kw["window"], kw["softcap"], None, 1,
-                        out, st, None, 0, 1, 1)
+                        out, st, None, 0, 1)
     if what in ("scale type", "int64 lengths", "bounds", "page", "code type", "devices"):
         with pytest.raises(ValueError, match="kv8_append"):
             C.kv8_append(c.k, c.v, c.k_scale, c.v_scale, a["k"], a["k"], a["table"], a["ctx"], a["cu"], 1, st)
@@ -694,7 +694,7 @@ def test_refusals_of_sums_and_eviction_need_no_gpu(what):
     if what in ("sums type", "sums shape", "rows overlap", "observe"):
         with pytest.raises(ValueError, match="kv8_attention"):
             C.kv8_attention(a["q"], c.k, c.v, c.k_scale, c.v_scale, a["table"], a["ctx"], a["cu"], 1, 0.1, 0, 0.0, None, 1,
-                            torch.zeros(1, 4, 32, dtype=torch.bfloat16), st, w, observe, 1, 1)
+                            torch.zeros(1, 4, 32, dtype=torch.bfloat16), st, w, observe, 1)
     if what != "observe":
         with pytest.raises(ValueError, match="kv8_evict"):
             C.kv8_evict(c.k, c.v, c.k_scale, c.v_scale, a["table"], a["ctx"], w, budget, first, last, dst, i32([0]),
