@@ -125,7 +125,8 @@ struct Pieces {
   }
 };
 
-template <int KH, int MT, int NQ, bool CAP>
+// SCORES: they are left in a.scores
+template <int KH, int MT, int NQ, bool CAP, bool SCORES>
 __global__ void __launch_bounds__(416, 1)
 kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const DecodeArgs p) {
   using C = Cfg<KH, MT, NQ>;
@@ -160,18 +161,13 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   const int G = p.a.Hq / c.Hkv, gtiles = (G + NQ - 1) / NQ, groups = c.Hkv * gtiles, n_seqs = p.s.n;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < ST; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_done[i], 1);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_done[i], 1);
-    }
-    for (int i = 0; i < 4; ++i) mbar_init(&p_ready[i], 128);
-    for (int i = 0; i < 2; ++i) mbar_init(&q_free[i], 1);
-    for (int i = 0; i < 8; ++i) mbar_init(&q_full[i], 32);
-    for (int i = 0; i < 16; ++i) mbar_init(&sc_full[i], 64);
-    *abort_flag = 0;
+  if (warp == 1) {                 // (one thread for all barriers took a microsecond)
+    if (lane < 24) mbar_init(bars + lane, 1);                            // stages
+    else if (lane < 28) mbar_init(bars + lane, 128);                     // p_ready
+    else if (lane < 30) mbar_init(bars + lane, 1);                       // q_free
+    if (lane < 8) mbar_init(&q_full[lane], 32);
+    else if (lane < 24) mbar_init(&sc_full[lane - 8], 64);
+    if (lane == 0) *abort_flag = 0;
     mbar_fence_init();
   }
   if (warp == 8) {
@@ -493,8 +489,11 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
         const int key0 = (tile0 + i - it) * BKV, tok = key0 + tl;
         const bool valid = tok >= start && tok < ctx;
-        const int rel = tok - s.i.tile0 * BKV;
-        float* sc_out = p.a.scores && rel < p.a.span ? p.a.scores + (long(row) * p.a.Hq + head0) * p.a.span + rel : nullptr;
+        float* sc_out = nullptr;
+        if constexpr (SCORES) {
+          const int rel = tok - s.i.tile0 * BKV;
+          if (valid && rel < p.a.span) sc_out = p.a.scores + (long(row) * p.a.Hq + head0) * p.a.span + rel;
+        }
         float z[NQ];
         bool over = false;
 #pragma unroll
@@ -503,7 +502,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           if (q < gn) {
             float x = fmaf(__uint_as_float(r[NQ + q]), 0.0625f, __uint_as_float(r[q])) * mul;
             if constexpr (CAP) x = fmaf(softcap_r(x, 1.f), p.scale_log2, 0.5f * p.scale_log2);
-            if (sc_out && valid) sc_out[q * long(p.a.span)] = x;
+            if (SCORES && sc_out) sc_out[q * long(p.a.span)] = x;
             if (valid) z[q] = x + add;
             over |= z[q] > m_ref[q] + SLACK;
           }
@@ -758,9 +757,9 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8Seqs s, const Kv
   join(a, D, row, h, n_splits, [&](int i) { return part + ((row * a.Hq + h) * n_splits + i) * (D + 2); }, s_w);
 }
 
-template <int KH, int MT, int NQ, bool CAP>
+template <int KH, int MT, int NQ, bool CAP, bool SCORES>
 cudaError_t launch(const CUtensorMap* tk, const CUtensorMap* tv, const DecodeArgs& p, int ctas, cudaStream_t st) {
-  auto kfn = kv8_decode_kernel<KH, MT, NQ, CAP>;
+  auto kfn = kv8_decode_kernel<KH, MT, NQ, CAP, SCORES>;
   constexpr int smem = Cfg<KH, MT, NQ>::SMEM;
   static DeviceOnce once;
   const cudaError_t e = once.shared_memory(reinterpret_cast<const void*>(kfn), smem);
@@ -794,8 +793,10 @@ int kv8_decode_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int
   }
   const int kh = (c.dk + 127) / 128, mt = (c.dv + 127) / 128, nq = kv8_decode_heads(a.Hq / c.Hkv);
   cudaError_t e = cudaErrorInvalidValue;
-#define LB_KV8(K_, V_, Q_) \
-  if (kh == K_ && mt == V_ && nq == Q_) e = cap ? launch<K_, V_, Q_, true>(tk, tv, p, ctas, st) : launch<K_, V_, Q_, false>(tk, tv, p, ctas, st);
+#define LB_KV8(K_, V_, Q_)                                                                                                      \
+  if (kh == K_ && mt == V_ && nq == Q_)                                                                                         \
+    e = a.scores ? (cap ? launch<K_, V_, Q_, true, true>(tk, tv, p, ctas, st) : launch<K_, V_, Q_, false, true>(tk, tv, p, ctas, st)) \
+                 : (cap ? launch<K_, V_, Q_, true, false>(tk, tv, p, ctas, st) : launch<K_, V_, Q_, false, false>(tk, tv, p, ctas, st));
   LB_KV8(1, 1, 8) LB_KV8(1, 1, 16) LB_KV8(2, 2, 8) LB_KV8(2, 2, 16) LB_KV8(1, 2, 8) LB_KV8(1, 2, 16) LB_KV8(2, 1, 8) LB_KV8(2, 1, 16)
 #undef LB_KV8
   if (e == cudaSuccess && ctas > 1) e = launch_pdl(kv8_combine_kernel, dim3(ctas, nq), dim3(128), 0, st, p, nq);
