@@ -38,7 +38,10 @@ struct PCfg {
   static constexpr int Q_BYTES = RT * 2 * KH * 16384;
   static constexpr int K_BYTES = KH * 16384, V8_BYTES = MT * 16384, V16_BYTES = MT * 32768;
   static constexpr int KS = 2, V8S = MT == 1 ? 2 : 1, V16S = MT == 1 ? 2 : 1;
-  static constexpr int TAIL = 2048;
+  // registers of a softmax thread and of the others: together what the launch has (512 x 128 or 384 x 168)
+  static constexpr int REGS_ROW = RT == 2 ? 184 : 232, REGS_REST = RT == 2 ? 72 : 136;
+  static_assert(RT * 128 * REGS_ROW + 256 * REGS_REST <= (RT == 2 ? 512 * 128 : 384 * 168), "registers");
+  static constexpr int TAIL = 1280 + RT * 512;
   static constexpr int SMEM = Q_BYTES + KS * K_BYTES + V8S * V8_BYTES + V16S * V16_BYTES + TAIL;
   static constexpr int O_COL = 256;      // score buffers at 0 and 128
   static_assert(SMEM <= 227 * 1024 && O_COL + RT * MT * 128 <= 512, "sizes");
@@ -92,49 +95,55 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+template <bool MASK, bool CAP, bool WIDE>
+__device__ __forceinline__ void part_row(const uint32_t (&r)[32], const float4* sc, float fq, float ref, float cap_scale, int lo, int hi,
+                                         uint32_t* w, float& mx0, float& mx1, float& total) {
+  constexpr int PER = WIDE ? 32 : 8;
+#pragma unroll
+  for (int e = 0; e < 32; e += PER) {
+    const float4 f = sc[e / 8];
+    const float mul = fq * f.x, add = CAP ? f.y + ref + 0.5f * cap_scale : f.y + ref;
+    const uint64_t mul2 = f2(mul, mul), add2 = f2(add, add);
+    uint64_t acc = f2(0.f, 0.f);
+#pragma unroll
+    for (int j = e; j < e + PER; j += 2) {
+      float z0, z1;
+      if constexpr (CAP) {
+        z0 = fmaf(softcap_r(__uint_as_float(r[j]) * mul, 1.f), cap_scale, add);
+        z1 = fmaf(softcap_r(__uint_as_float(r[j + 1]) * mul, 1.f), cap_scale, add);
+      } else {
+        f2_out(f2_fma(f2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), mul2, add2), z0, z1);
+      }
+      if constexpr (MASK) {
+        if (j < lo || j >= hi) z0 = -INFINITY;
+        if (j + 1 < lo || j + 1 >= hi) z1 = -INFINITY;
+      }
+      if (j & 2) mx1 = fmax3(mx1, z0, z1);
+      else mx0 = fmax3(mx0, z0, z1);
+      const float y0 = ex2(z0), y1 = ex2(z1);
+      acc = f2_add(acc, f2(y0, y1));
+      w[j / 2] = half2_of(y0, y1);
+    }
+    float a0, a1;
+    f2_out(acc, a0, a1);
+    total = fmaf(a0 + a1, f.z, total);
+  }
+}
+
 // One row of a tile: w = halves of 2^(z + ref), their sum with every value scale divided out, and the largest z + ref. WIDE: a
 // scale for 32 keys or more, else for 8. MASK: keys outside [lo, hi) of the tile count nothing.
 template <bool MASK, bool CAP, bool WIDE>
 __device__ __forceinline__ void row_of_tile(uint32_t my_S, const float4* sc, float fq, float ref, float cap_scale, int lo, int hi,
                                             uint32_t (&w)[64], float& top, float& total) {
-  constexpr int PER = WIDE ? 32 : 8;
   float mx0 = -INFINITY, mx1 = -INFINITY;
   total = 0.f;
+  uint32_t r[2][32];
+  tmem_ld32(my_S, r[0]);
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    uint32_t r[32];
-    tmem_ld32(my_S + g * 32, r);
     tmem_ld_wait();
-#pragma unroll
-    for (int e = 0; e < 32; e += PER) {
-      const float4 f = sc[(g * 32 + e) / 8];
-      const float mul = fq * f.x, add = CAP ? f.y + ref + 0.5f * cap_scale : f.y + ref;
-      const uint64_t mul2 = f2(mul, mul), add2 = f2(add, add);
-      uint64_t acc = f2(0.f, 0.f);
-#pragma unroll
-      for (int j = e; j < e + PER; j += 2) {
-        float z0, z1;
-        if constexpr (CAP) {
-          z0 = fmaf(softcap_r(__uint_as_float(r[j]) * mul, 1.f), cap_scale, add);
-          z1 = fmaf(softcap_r(__uint_as_float(r[j + 1]) * mul, 1.f), cap_scale, add);
-        } else {
-          f2_out(f2_fma(f2(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), mul2, add2), z0, z1);
-        }
-        if constexpr (MASK) {
-          const int key = g * 32 + j;
-          if (key < lo || key >= hi) z0 = -INFINITY;
-          if (key + 1 < lo || key + 1 >= hi) z1 = -INFINITY;
-        }
-        if (j & 2) mx1 = fmax3(mx1, z0, z1);
-        else mx0 = fmax3(mx0, z0, z1);
-        const float y0 = ex2(z0), y1 = ex2(z1);
-        acc = f2_add(acc, f2(y0, y1));
-        w[(g * 32 + j) / 2] = half2_of(y0, y1);
-      }
-      float a0, a1;
-      f2_out(acc, a0, a1);
-      total = fmaf(a0 + a1, f.z, total);
-    }
+    if (g < 3) tmem_ld32(my_S + g * 32 + 32, r[(g + 1) & 1]);      // on its way while this one is worked on
+    part_row<MASK, CAP, WIDE>(r[g & 1], sc + g * 4, fq, ref, cap_scale, lo - g * 32, hi - g * 32, w + g * 16, mx0, mx1, total);
   }
   top = fmaxf(mx0, mx1);
 }
@@ -170,6 +179,8 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   int* s_nan = reinterpret_cast<int*>(bars + 24);       // first and last key with a NaN value, then a bit per column [8]
   float4* s_sc = reinterpret_cast<float4*>(bars + 32);  // [4][16]: key scale, log2 of the value scale 2^e, 2^-e, per 8 keys
 
+  float* s_q = reinterpret_cast<float*>(bars + 160);    // [RT * 128]: a row's power of two times the score scale
+
   const Kv8Cache& c = p.c;
   const int G = p.a.Hq / c.Hkv;
   const int kvh = blockIdx.y % c.Hkv, split = blockIdx.y / c.Hkv, seq = blockIdx.z;
@@ -195,7 +206,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   const int wg = warp >> 2;                             // < RT: softmax, RT: values, RT + 1: TMA and MMA
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, RT * 128);
+    mbar_init(q_full, (RT + 1) * 128);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -224,7 +235,65 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   const uint32_t tmem = *tmem_slot;
   auto fail = [&](int code) { *abort_flag = 1; atomicCAS(p.s.status, 0, code | SITE_PREFILL_ATTN); return false; };
 
+  // Queries, by the softmax and the value warps, a row at a time: a power of two, two e4m3 terms. Not finite: a NaN code.
+  if (wg <= RT) {
+    const int dims = KH * 4;                            // of a lane
+#pragma unroll 4
+    for (int r = warp; r < RT * 128; r += (RT + 1) * 4) {
+      const int gr = row0 + r;
+      uint32_t u[KH * 2];
+#pragma unroll
+      for (int k = 0; k < KH * 2; ++k) u[k] = 0u;
+      if (r < rows && lane * dims < c.dk) {
+        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + (long(q0) + gr / G) * p.a.q_tok + (kvh * G + gr % G) * p.a.q_head +
+                                   lane * dims;
+        if ((reinterpret_cast<uintptr_t>(src) & (KH * 8 - 1)) == 0) {
+          if (KH == 1) *reinterpret_cast<uint2*>(u) = *reinterpret_cast<const uint2*>(src);
+          else *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(src);
+        } else {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+          for (int k = 0; k < KH * 2; ++k) u[k] = h[2 * k] | uint32_t(h[2 * k + 1]) << 16;
+        }
+      }
+      uint32_t m = 0;
+#pragma unroll
+      for (int k = 0; k < KH * 2; ++k) {
+        const uint32_t lo = u[k] & 0x7fffu, hi = (u[k] >> 16) & 0x7fffu;
+        m = max(m, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+      }
+      m = __reduce_max_sync(0xffffffffu, m);
+      const float qs = kv8_scale_of(__uint_as_float(m << 16)), inv = kv8_inverse(qs);
+      if (lane == 0) s_q[r] = qs * (CAP ? p.cap_k : p.scale_log2);
+      uint32_t hi4[KH], lo4[KH];
+#pragma unroll
+      for (int k = 0; k < KH * 2; ++k) {
+        const float a0 = __uint_as_float(u[k] << 16) * inv, a1 = __uint_as_float(u[k] & 0xffff0000u) * inv;
+        uint32_t hh = e4m3x2(a0, a1);
+        if ((u[k] & 0x7f80u) == 0x7f80u) hh |= 0x7fu;
+        if ((u[k] & 0x7f800000u) == 0x7f800000u) hh |= 0x7f00u;
+        const float2 f = __half22float2(e4m3x2_to_half2(hh));
+        // the remainder in the units of the first term: its lower end, 2^-10 of a largest code of 128 or more, is 2^-17 of the row's
+        // largest value; bf16 values that small have a step of 2^-9 of themselves
+        const uint32_t ll = e4m3x2(a0 - f.x, a1 - f.y);
+        if (k & 1) { hi4[k / 2] |= hh << 16; lo4[k / 2] |= ll << 16; }
+        else { hi4[k / 2] = hh; lo4[k / 2] = ll; }
+      }
+      const int d = lane * dims, ch = d / 16;
+      uint8_t* dst = q_s + ((r / 128) * 2 * KH + ch / 8) * 16384 + (r % 128) * 128 + (((ch & 7) ^ (r & 7)) << 4) + d % 16;
+      if (KH == 1) {
+        *reinterpret_cast<uint32_t*>(dst) = hi4[0];
+        *reinterpret_cast<uint32_t*>(dst + KH * 16384) = lo4[0];
+      } else {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(hi4[0], hi4[KH - 1]);
+        *reinterpret_cast<uint2*>(dst + KH * 16384) = make_uint2(lo4[0], lo4[KH - 1]);
+      }
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(q_full);
+  }
   if (wg == RT + 1) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_REST));
     if (warp == (RT + 1) * 4 + 1) {
       // ---------------------------------------------------------------- TMA: the lanes fetch table and scales, lane 0 issues
       const int* bt = p.s.table + seq * p.s.ld_table;
@@ -326,6 +395,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
   } else if (wg == RT) {
     // ------------------------------------------------------------------ values: e4m3 -> half, thread = key
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_REST));
     const int key = threadIdx.x - RT * 128;
     bool ok = true;
     for (int i = 0; i < n_tiles; ++i) {
@@ -386,6 +456,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
   } else {
     // ------------------------------------------------------------------ softmax, thread = row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_ROW));
     const int row = threadIdx.x & 127;
     const int gr = row0 + wg * 128 + row;
     const bool row_ok = wg * 128 + row < rows;
@@ -393,63 +464,13 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const long t = long(q0) + tok_row;
     const int pos = ctx - n_new + tok_row;
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
-    float fq;
-    {
-      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + (row_ok ? t * p.a.q_tok + head * p.a.q_head : 0);
-      const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-      auto load8 = [&](int d) -> uint4 {
-        if (!row_ok || d >= c.dk) return make_uint4(0u, 0u, 0u, 0u);
-        if (vec) return *reinterpret_cast<const uint4*>(src + d);
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(src + d);
-        return make_uint4(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16, h[4] | uint32_t(h[5]) << 16, h[6] | uint32_t(h[7]) << 16);
-      };
-      uint32_t m = 0;
-#pragma unroll 4
-      for (int d = 0; d < c.dk; d += 8) {
-        const uint4 u = load8(d);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t lo = w[j] & 0x7fffu, hi = (w[j] >> 16) & 0x7fffu;
-          m = max(m, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-        }
-      }
-      const float qs = kv8_scale_of(__uint_as_float(m << 16)), inv = kv8_inverse(qs);
-      fq = qs * (CAP ? p.cap_k : p.scale_log2);
-#pragma unroll 2
-      for (int ch = 0; ch < KH * 8; ++ch) {
-        uint32_t hi4[4], lo4[4];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint4 u = load8(ch * 16 + half * 8);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float a0 = __uint_as_float(w[j] << 16) * inv, a1 = __uint_as_float(w[j] & 0xffff0000u) * inv;
-            uint32_t hh = e4m3x2(a0, a1);
-            if ((w[j] & 0x7f80u) == 0x7f80u) hh |= 0x7fu;            // not finite: NaN
-            if ((w[j] & 0x7f800000u) == 0x7f800000u) hh |= 0x7f00u;
-            const float2 f = __half22float2(e4m3x2_to_half2(hh));
-            // the remainder in the units of the first term: its lower end, 2^-10 of a largest code of 128 or more, is 2^-17 of
-            // the row's largest value; bf16 values that small have a step of 2^-9 of themselves
-            const uint32_t ll = e4m3x2(a0 - f.x, a1 - f.y);
-            const int k = half * 2 + j / 2;
-            if (j & 1) { hi4[k] |= hh << 16; lo4[k] |= ll << 16; }
-            else { hi4[k] = hh; lo4[k] = ll; }
-          }
-        }
-        uint8_t* dst = q_s + (wg * 2 * KH + ch / 8) * 16384 + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
-        *reinterpret_cast<uint4*>(dst) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
-        *reinterpret_cast<uint4*>(dst + KH * 16384) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(q_full);
-    }
+    bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, abort_flag));
+    if (!ok) fail(ST_TIMEOUT_FULL);
+    const float fq = s_q[wg * 128 + row];
     const int hi = row_ok ? min(ctx, pos + 1) : 0, lo = p.a.window > 0 ? max(0, pos - p.a.window + 1) : 0;
     const uint32_t my_O = tmem + C::O_COL + wg * (MT * 128) + lane_off;
     float m = -INFINITY, l = 0.f;
-    bool ok = true;
-    if (wg < n_rt) {
+    if (ok && wg < n_rt) {
       for (int i = 0; i < n_tiles; ++i) {
         const int u = i * n_rt + wg, b = u & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&sc_full[i & 3], (i >> 2) & 1, abort_flag)) &&
