@@ -36,6 +36,8 @@ def _add_engine_args(ap: argparse.ArgumentParser):
                    help="share of the device's memory the memory plan may fill")
     g.add_argument("--kv-block", type=int, default=None, help="tokens per KV block (64 on GPU, 16 on CPU)")
     g.add_argument("--no-prefix-cache", action="store_true")
+    g.add_argument("--kv-dtype", choices=("auto", "fp8"), default="auto",
+                   help="auto: keys and values as the model computes them; fp8: 8 bits with a scale per block of tokens and head")
     g.add_argument("--kv-rings", action="store_true",
                    help="sliding-window layers keep window + one step of K / V per sequence in a ring of blocks instead "
                         "of pages for the whole context (prompts then resume from the prefix cache at state snapshots only)")
@@ -150,6 +152,7 @@ def build_engine_from_args(a, start: bool = True):
         kv_cache_tokens=a.kv_cache_tokens,
         gpu_memory_utilization=getattr(a, "gpu_memory_utilization", None) or hd.gpu_memory_utilization or 0.92,
         kv_fit_check=True, prefix_cache=not a.no_prefix_cache, kv_rings=getattr(a, "kv_rings", False),
+        kv_dtype=getattr(a, "kv_dtype", "auto"),
         prefix_cache_states=a.prefix_cache_states, prefix_cache_interval=a.prefix_cache_interval,
         max_waiting=a.max_waiting, default_max_tokens=a.default_max_tokens, scheduling_policy=a.scheduling_policy,
         fair_share=a.fair_share, kv_admission=a.kv_admission, spec=a.spec, spec_k=a.spec_k, spec_draft_model=getattr(a, "spec_draft_model", None),

@@ -47,6 +47,7 @@ class EngineConfig:
     max_batch_tokens: int = 1024
     prefill_chunk: int = 512
     block_size: int = 64
+    kv_dtype: str = "auto"                      # auto: the model's; fp8: e4m3 with a scale per block and head (ops.Kv8Cache)
     kv_cache_tokens: Optional[int] = None       # None: max_seqs * ctx_size; -1: as many as fit the GPU (memory plan)
     gpu_memory_utilization: float = 0.92        # share of the device's memory the memory plan may fill
     kv_fit_check: bool = False                  # refuse to start when an explicit KV pool does not fit
@@ -175,6 +176,14 @@ class LmEngine(Engine):
         # the state snapshots (``StatePool.attach_rings``), so a prompt resumes from the cache only where a snapshot
         # exists, as for recurrent layers. Preempted sequences are recomputed.
         self.ring_len = 0
+        if c.kv_dtype not in ("auto", "fp8"):
+            raise ValueError(f"kv_dtype is auto or fp8, not {c.kv_dtype}")
+        kv8 = c.kv_dtype == "fp8"
+        if kv8:
+            if self.dp_world > 1 or getattr(model, "pipe", None) is not None or c.kv_rings:
+                raise ValueError("an 8-bit KV cache is not available with data-parallel attention, pipeline stages or window rings")
+            c.kv_swap_gib = 0.0                 # preempted sequences are recomputed, evicted prefixes dropped
+            c.prefix_host_gib = 0.0
         if c.kv_rings and "swa" in self.mcfg.layer_kinds and self.mcfg.sliding_window > 0:
             if self.dp_world > 1 or getattr(model, "pipe", None) is not None:
                 raise ValueError("sliding-window rings are not available with data-parallel attention or pipeline stages")
@@ -194,7 +203,7 @@ class LmEngine(Engine):
         self.snap_resume = self.hybrid or bool(self.ring_len)
         n_saved = c.prefix_cache_states if (self.snap_resume and c.prefix_cache) else 0
         self.kv = KvCache(self.mcfg, n_blocks, c.block_size, dev, model.dtype, kv_heads_local=model.n_kv_l,
-                          extra_layers=extra, owns=owns, ring_blocks=self.ring_len * (c.max_seqs + n_saved + 1))
+                          extra_layers=extra, owns=owns, ring_blocks=self.ring_len * (c.max_seqs + n_saved + 1), kv8=kv8)
         self.states = (StatePool(self.mcfg, c.max_seqs + n_saved + 1, dev, tp=model.pctx.tp, owns=owns)
                        if self.snap_resume else None)
         if self.ring_len:
@@ -252,7 +261,7 @@ class LmEngine(Engine):
         from . import memory_plan as mp
         c = self.cfg
         probe = KvCache(self.mcfg, 1, c.block_size, dev, model.dtype, kv_heads_local=model.n_kv_l, extra_layers=extra,
-                        owns=owns)
+                        owns=owns, kv8=c.kv_dtype == "fp8")
         bpb = probe.bytes_per_block()
         bpb_ring = probe.bytes_per_block(swa_only=True) if self.ring_len else 0
         del probe

@@ -68,6 +68,7 @@ class StepBatch:
     block_table_ring: Optional[torch.Tensor] = None  #   block table (logical block j -> ring block j mod ring length)
     deepstack_rows: Optional[torch.Tensor] = None    # [R] int64 rows of this step that are image tokens, and per early
     deepstack: Optional[List[torch.Tensor]] = None   #   layer the [R, hidden] rows added to the stream after it
+    kv8_rows: Optional[tuple] = None             # 8-bit cache: (lengths, 0 where a sequence's rows are padding; arange(T))
 
     @property
     def n_seqs(self) -> int:
@@ -86,10 +87,15 @@ class KvCache:
     """Per-layer paged K/V tensors ``[n_blocks, page, kv_heads, dim]`` (MLA layers: one latent row)."""
 
     def __init__(self, cfg: ModelConfig, n_blocks: int, page: int, device, dtype, kv_heads_local: Optional[int] = None,
-                 extra_layers: int = 0, owns=None, ring_blocks: int = 0):
+                 extra_layers: int = 0, owns=None, ring_blocks: int = 0, kv8: bool = False):
         """``ring_blocks`` > 0: sliding-window layers keep their K / V in a pool of that many blocks of their own
-        (a short ring of blocks per sequence slot, ``engine.lm``) instead of ``n_blocks``."""
-        self.page, self.n_blocks = page, n_blocks
+        (a short ring of blocks per sequence slot, ``engine.lm``) instead of ``n_blocks``. ``kv8``: keys and values in 8 bits
+        with a scale per block and head (``ops.Kv8Cache``, the same object under ``k`` and ``v``)."""
+        self.page, self.n_blocks, self.kv8 = page, n_blocks, kv8
+        if kv8 and (cfg.layers is not None or cfg.kv_lora > 0 or cfg.sandwich_norm or cfg.block_form or cfg.hyper_streams > 1
+                    or "mla" in cfg.layer_kinds or cfg.head_dim % 16 or ring_blocks):
+            raise ValueError("an 8-bit KV cache is for models whose attention layers keep plain keys and values of 16, 32, .. 256 "
+                             "columns, without window rings")
         self.ring_blocks = ring_blocks
         self._kinds = tuple(cfg.layer_kinds)
         self.k: Dict[int, torch.Tensor] = {}
@@ -117,6 +123,9 @@ class KvCache:
                 self.v[il] = torch.zeros(nb, page, hk, d, device=device, dtype=dtype)
             else:
                 hk = kv_heads_local or cfg.n_kv_head
+                if kv8:
+                    self.k[il] = self.v[il] = ops.Kv8Cache.empty(n_blocks, page, hk, cfg.head_dim, device=device)
+                    continue
                 nb = ring_blocks if (ring_blocks and kinds[il] == "swa") else n_blocks
                 self.k[il] = torch.zeros(nb, page, hk, cfg.head_dim, device=device, dtype=dtype)
                 self.v[il] = torch.zeros(nb, page, hk, cfg.head_dim, device=device, dtype=dtype)
@@ -129,6 +138,8 @@ class KvCache:
     def bytes_per_block(self, swa_only: bool = False) -> int:
         """Bytes one block takes over every layer that owns a cache; ``swa_only`` counts the sliding-window layers
         alone (the part that moves into per-slot rings when ring storage is on)."""
+        if self.kv8:
+            return sum(k.bytes_per_block() for k in self.k.values())
         n = 0
         seen = set()
         kinds = self._kinds
@@ -146,9 +157,13 @@ class KvCache:
     def copy_blocks(self, src: List[int], dst: List[int]):
         if not src:
             return
-        s = torch.tensor(src, device=next(iter(self.k.values())).device)
+        first = next(iter(self.k.values()))
+        s = torch.tensor(src, device=(first.k if self.kv8 else first).device)
         d = torch.tensor(dst, device=s.device)
         for il in self.k:
+            if self.kv8:
+                self.k[il].copy_blocks(s, d)
+                continue
             self.k[il][d] = self.k[il][s]
             if self.v[il] is not self.k[il]:
                 self.v[il][d] = self.v[il][s]
@@ -493,11 +508,23 @@ class Decoder:
         slots, table = b.slots, b.block_table
         if window > 0 and b.slots_ring is not None:
             slots, table = b.slots_ring, b.block_table_ring      # this layer's K / V live in the sequence's ring
+        k_new, v_new = kv.k[il], kv.v[il]
+        if kv.kv8:
+            # this step's keys and values as a cache of one block: they are encoded when all of a block's are there
+            rows = b.kv8_rows or self._kv8_rows(b)
+            k_new, v_new = torch.empty(2, 1, qkv.shape[0], self.n_kv_l, D, dtype=qkv.dtype, device=qkv.device)
+            slots = rows[1]
         q, gate = ops.qk_norm_rope_append(qkv, self.n_head_l, self.n_kv_l, D, w.get(f"{p}.attn.q_norm"),
                                           w.get(f"{p}.attn.k_norm"), cfg.rms_eps, cfg.norm_offset, cos_sin,
-                                          cfg.rope_dim if rope else 0, positions, slots, kv.k[il], kv.v[il],
+                                          cfg.rope_dim if rope else 0, positions, slots, k_new, v_new,
                                           cfg.gated_attn)
         scale = cfg.attn_scale or D ** -0.5
+        if kv.kv8:
+            ops.kv8_append(kv.k[il], k_new[0], v_new[0], table, rows[0], b.cu_q, b.max_q_len)
+            o = ops.kv8_attention(q, kv.k[il], table, rows[0], b.cu_q, b.max_q_len, scale, window=window, max_ctx=b.max_ctx or None)
+            if cfg.gated_attn:
+                o = ops.apply_output_gate(o, gate, self.n_head_l, D)
+            return self.pctx.defer_linear(o.reshape(o.shape[0], -1), w[f"{p}.attn.o"], lazy=True)
         o = ops.paged_attention(q, kv.k[il], kv.v[il], table, b.ctx_lens, b.cu_q, b.max_q_len, scale,
                                 window=window, decode_splits=b.decode_splits, max_ctx=b.max_ctx or None)
         if cfg.gated_attn:
@@ -1640,7 +1667,15 @@ class Decoder:
         pc.end_step()
         return StepOutput(hidden=hidden, logits=logits, last_hidden=last, captures={})
 
+    @staticmethod
+    def _kv8_rows(b: StepBatch):
+        """Lengths with 0 for sequences whose rows are padding (slot -1: their table is not theirs), and arange(T)."""
+        last = b.slots[(b.cu_q[1:] - 1).clamp_min(0).long()]
+        return torch.where(last >= 0, b.ctx_lens, torch.zeros_like(b.ctx_lens)), torch.arange(b.slots.shape[0], device=b.slots.device)
+
     def forward(self, b: StepBatch, kv: KvCache, st: Optional[StatePool], want_logits: bool = True) -> StepOutput:
+        if kv.kv8:
+            b.kv8_rows = self._kv8_rows(b)           # (made anew in every call, so that a captured step does, too)
         if self.pipe is not None:
             return self._forward_pipe(b, kv, st, want_logits)
         if self.cfg.layers is not None:

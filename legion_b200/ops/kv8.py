@@ -42,6 +42,11 @@ class Kv8Cache:
     def page(self) -> int:
         return self.k.shape[2]
 
+    def copy_blocks(self, src, dst):
+        """Blocks ``src`` (int64) to blocks ``dst``."""
+        for t in (self.k.view(torch.uint8), self.v.view(torch.uint8), self.k_scale, self.v_scale):
+            t[dst] = t[src]
+
     def bytes_per_block(self) -> int:
         return self.k[0].numel() + self.v[0].numel() + 8 * self.k.shape[1]
 

@@ -619,6 +619,105 @@ def test_a_chat_whose_cache_is_pruned(device):
     assert status(device) == 0
 
 
+# ------------------------------------------------------------------------------------- streams, graphs, many launches
+@gpu
+def test_two_streams_at_once():
+    """Calls on two streams share no scratch: each gives what it gives alone."""
+    device, cases = "cuda:0", []
+    for j, (lens, new) in enumerate((([3000, 500, 77], [1, 1, 1]), ([900, 1500, 60], [300, 5, 60]))):
+        cache, table = filled(lens, 16, 2, 64, 64, seed=j, device=device)
+        q = randn(sum(new), 8, 64, seed=j + 9).bfloat16().to(device)
+        args = (q, cache, i32(table, device), i32(lens, device), i32(cum(new), device), max(new), 0.125)
+        w = torch.zeros(3, 2, max(lens), device=device)
+        cases.append((args, ops.kv8_attention(*args, weights=w).clone(), w))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for j in (0, 1):
+            with torch.cuda.stream(streams[j]):
+                w = torch.zeros_like(cases[j][2])
+                got[j].append((ops.kv8_attention(*cases[j][0], weights=w), w))
+    torch.cuda.synchronize()
+    for j in (0, 1):
+        for o, w in got[j]:
+            assert torch.equal(o, cases[j][1]) and torch.equal(w, cases[j][2])
+    assert status(device) == 0
+
+
+@gpu
+def test_captured_and_replayed_with_new_data():
+    """Append, attention with sums and eviction in two graphs that are replayed in turn, lengths and rows changed between replays."""
+    device, page, kv, heads, D = "cuda:0", 16, 2, 8, 64
+    graphs = []
+    for j in range(2):
+        cache = ops.Kv8Cache.empty(40, page, kv, D, D, device)
+        table, dst = i32([list(range(1, 9)), list(range(9, 17))], device), i32([[20, 21], [22, 23]], device)
+        ctx, cu = i32([40, 20], device), i32([0, 1, 2], device)
+        k, v, q = (torch.zeros(2, h, D, dtype=torch.bfloat16, device=device) for h in (kv, kv, heads))
+        sums = torch.zeros(2, kv, 128, device=device)
+
+        def body():
+            ops.kv8_append(cache, k, v, table, ctx, cu, 1)
+            o = ops.kv8_attention(q, cache, table, ctx, cu, 1, 0.2, weights=sums)
+            return (o,) + ops.kv8_evict(cache, table, ctx, sums, 24, dst, keep_first=2, keep_last=4)
+        fill = randn(60, kv, D, seed=j).bfloat16().to(device)
+        ops.kv8_append(cache, fill, fill, table, i32([39, 19], device), i32([0, 39, 58], device), 39)
+        body()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = body()
+        graphs.append((g, out, cache, (k, v, q), ctx, sums, table, (cu, dst)))      # (a graph keeps no tensor alive)
+    for step in range(3):
+        for j, (g, out, cache, rows, ctx, sums, table, _) in enumerate(graphs):
+            for t, h in zip(rows, (kv, kv, heads)):
+                t.copy_(randn(2, h, D, seed=100 * step + 10 * j + h))
+            lens = [41 + step, 21 + step]
+            ctx.copy_(i32(lens))
+            sums.zero_()
+            before = on(cache, "cpu")
+            g.replay()
+            torch.cuda.synchronize()
+            ops.kv8_append(before, rows[0].cpu(), rows[1].cpu(), table.cpu(), i32(lens), i32([0, 1, 2]), 1)
+            want, tol, weight, off = attend(rows[2].cpu(), before, table.tolist(), lens, [1, 1], 0.2)
+            near(out[0], want, tol)
+            assert out[1].tolist() == [24, min(24, lens[1])]
+            for i, n in enumerate(lens):
+                assert bool(((sums[i, :, :n].cpu().double() - weight[i].sum(2)).abs() <= off[i].sum(2) + 2.0 ** -22).all())
+                kept = out[2][i, 0, :min(24, n)].tolist()
+                assert kept == sorted(kept) and kept[:2] == [0, 1] and kept[-4:] == list(range(n - 4, n))
+    assert status(device) == 0
+
+
+@gpu
+def test_the_same_call_gives_the_same_bits():
+    device = "cuda:0"
+    lens, new = [2000, 300, 1, 129], [1, 1, 1, 1]
+    cache, table = filled(lens, 64, 2, 128, 128, seed=1, device=device)
+    q = randn(4, 16, 128, seed=2).bfloat16().to(device)
+    first = None
+    for _ in range(10):
+        w = torch.zeros(4, 2, 2000, device=device)
+        o = ops.kv8_attention(q, cache, i32(table, device), i32(lens, device), i32(cum(new), device), 1, 0.1, weights=w)
+        first = first or (o, w)
+        assert torch.equal(o, first[0]) and torch.equal(w, first[1])
+
+
+@gpu
+def test_empty_calls():
+    device = "cuda:0"
+    cache, table = filled([20], 16, 2, 32, 32, device=device)
+    none = torch.empty(0, 4, 32, dtype=torch.bfloat16, device=device)
+    o = ops.kv8_attention(none, cache, i32(table, device), i32([20], device), i32([0, 0], device), 0, 1.0)
+    assert o.shape == (0, 4, 32)
+    ops.kv8_append(cache, none[:, :2], none[:, :2], i32(table, device), i32([20], device), i32([0, 0], device), 0)
+    no_seqs = torch.empty(0, 3, dtype=torch.int32, device=device)
+    o = ops.kv8_attention(none, cache, no_seqs, i32([], device), i32([0], device), 0, 1.0)
+    lens, kept, sums = ops.kv8_evict(cache, no_seqs, i32([], device), torch.empty(0, 2, 5, device=device), 4, no_seqs)
+    assert lens.shape == (0,) and kept.shape == (0, 2, 4) and status(device) == 0
+
+
 # -------------------------------------------------------------------------------------------------------- refusals
 def _refusals():
     def base():
