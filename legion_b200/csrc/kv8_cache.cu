@@ -57,21 +57,17 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
   const int col = first / c.page + j;
   const int lo = max(first, col * c.page), hi = min(ctx, (col + 1) * c.page);
   if (n <= 0 || lo >= hi) return;
-  const int blk = p.s.table[b * p.s.ld_table + col];
-  if (unsigned(blk) >= unsigned(c.n_blocks) || row0 < 0 || long(row0) + n > p.s.T || n > p.s.max_new) {
+  if (row0 < 0 || long(row0) + n > p.s.T || n > p.s.max_new) {
     if (threadIdx.x == 0) atomicCAS(p.s.status, 0, ST_BAD_ARGS);
     return;
   }
+  const int blk = p.s.table[b * p.s.ld_table + col];
   const int D = val ? c.dv : c.dk, per = D / 8;
   const long tok = val ? p.a.v_tok : p.a.k_tok;
   const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(val ? p.a.v : p.a.k) + (val ? p.a.v_head : p.a.k_head) * h +
                              (row0 + (lo - (ctx - n))) * tok;
-  const long unit = long(blk) * c.Hkv + h;
-  uint8_t* codes = (val ? c.v : c.k) + unit * c.page * D;
-  float* scale = (val ? c.v_scale : c.k_scale) + unit;
   const int nvec = (hi - lo) * per;
-  const float old = lo == col * c.page ? 0.f : *scale;
-  uint4 x[VPT];
+  uint4 x[VPT];                                             // on their way while the table answers
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
@@ -80,6 +76,14 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
       x[i] = load_row8(src + (at / per) * tok + (at % per) * 8, p.vec);
     }
   }
+  if (unsigned(blk) >= unsigned(c.n_blocks)) {
+    if (threadIdx.x == 0) atomicCAS(p.s.status, 0, ST_BAD_ARGS);
+    return;
+  }
+  const long unit = long(blk) * c.Hkv + h;
+  uint8_t* codes = (val ? c.v : c.k) + unit * c.page * D;
+  float* scale = (val ? c.v_scale : c.k_scale) + unit;
+  const float old = lo == col * c.page ? 0.f : *scale;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     if (threadIdx.x + i * APPEND_THREADS < nvec) m = max(max(m, max(mag2(x[i].x), mag2(x[i].y))), max(mag2(x[i].z), mag2(x[i].w)));
