@@ -5,18 +5,20 @@
 // per kv head, where scores made anew would read all keys again), and kv8_score_sums_kernel adds them up, a thread per key.
 //
 // Rows of a prompt: the scores once more. kv8_queries_kernel packs the rows that count, 64 (token, head) rows of a kv head to a
-// record: their two e4m3 terms in the layout that the MMA reads, one power of two, log-sum-exps and positions. kv8_weights_kernel,
+// record: their two e4m3 terms in the layout that the MMA reads, powers of two, log-sum-exps and positions. kv8_weights_kernel,
 // a CTA per 256 keys of a kv head, keeps its two key tiles in shared memory and streams the records past them:
-// S^T[128 keys, 2 x 64 rows] = K . Q^T on tcgen05; a thread has a key and adds up its columns over all records, so nothing crosses
-// threads and the result does not depend on any order but the rows' own. 64 exponentials per key and record bound it.
+// S^T[128 keys, 64 rows] = K . Q^T on tcgen05, with the terms, scales and order of the attention, whose sums its scores have to be
+// bit for bit: the tensor cores cut off what does not fit a sum, and scores summed in another order gave weights 10^-6 too large.
+// A thread has a key and adds up its columns over all records, so nothing crosses threads and the result does not depend on any
+// order but the rows' own. 64 exponentials per key and record bound it.
 #include "kv8_dev.cuh"
 #include "tmap.cuh"
 
 namespace lb {
 namespace {
 
-constexpr int RN = 64, NS = 2 * RN, BKV = 128;
-constexpr int HEAD = 1024;               // of a record: power of two, log-sum-exps (float 16 ..), positions (float 80 ..); codes behind it
+constexpr int RN = 64, BKV = 128;
+constexpr int HEAD = 1024;               // of a record: powers of two [64], log-sum-exps [64], positions [64]; behind it the first, then the second terms
 
 struct WeightArgs {
   Kv8Cache c;
@@ -49,88 +51,80 @@ __device__ __forceinline__ Rows rows_of(const WeightArgs& p, int seq, int G) {
 
 template <int KH>
 __global__ void __launch_bounds__(256) kv8_queries_kernel(const WeightArgs p) {
-  __shared__ uint32_t s_max[8];
   griddep_wait();
   griddep_launch();
   const int G = p.a.Hq / p.c.Hkv, rt = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
   const Rows x = rows_of(p, seq, G);
   const int n = min(RN, x.rows - rt * RN);
   if (n <= 0) return;
-  uint8_t* rec = p.records + ((long(seq) * p.c.Hkv + kvh) * p.max_rt + rt) * (HEAD + KH * NS * 128);
+  uint8_t* rec = p.records + ((long(seq) * p.c.Hkv + kvh) * p.max_rt + rt) * (HEAD + 2 * KH * RN * 128);
+  float* head = reinterpret_cast<float*>(rec);
   constexpr int PER = RN * KH * 8 / 256;                  // chunks of 16 values of a thread
-  uint32_t u[PER][8];
-  uint32_t m = 0;
-#pragma unroll
+#pragma unroll 1
   for (int j = 0; j < PER; ++j) {
-    const int i = threadIdx.x + j * 256, r = i / (KH * 8), ch = i % (KH * 8);
+    const int i = threadIdx.x + j * 256, r = i / (KH * 8), ch = i % (KH * 8);      // a row's chunks lie in neighbouring lanes
+    uint32_t u[8];
+    uint32_t m = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) u[j][k] = 0u;
+    for (int k = 0; k < 8; ++k) u[k] = 0u;
     if (r < n && ch * 16 < p.c.dk) {
       const int gr = rt * RN + r;
       const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + long(x.q0 + x.first + gr / G) * p.a.q_tok +
                                  (kvh * G + gr % G) * p.a.q_head + ch * 16;
       if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-        *reinterpret_cast<uint4*>(u[j]) = reinterpret_cast<const uint4*>(src)[0];
-        *reinterpret_cast<uint4*>(u[j] + 4) = reinterpret_cast<const uint4*>(src)[1];
+        *reinterpret_cast<uint4*>(u) = reinterpret_cast<const uint4*>(src)[0];
+        *reinterpret_cast<uint4*>(u + 4) = reinterpret_cast<const uint4*>(src)[1];
       } else {
         const uint16_t* hs = reinterpret_cast<const uint16_t*>(src);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) u[j][k] = hs[2 * k] | uint32_t(hs[2 * k + 1]) << 16;
+        for (int k = 0; k < 8; ++k) u[k] = hs[2 * k] | uint32_t(hs[2 * k + 1]) << 16;
       }
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const uint32_t lo = u[j][k] & 0x7fffu, hi = (u[j][k] >> 16) & 0x7fffu;
+      const uint32_t lo = u[k] & 0x7fffu, hi = (u[k] >> 16) & 0x7fffu;
       m = max(m, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
     }
-  }
-  m = __reduce_max_sync(0xffffffffu, m);
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
-  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, s_max[i]);
-  const float qs = kv8_scale_of(__uint_as_float(m << 16)), inv = kv8_inverse(qs);
-  float* head = reinterpret_cast<float*>(rec);
-  if (threadIdx.x == 0) head[0] = qs * (p.a.softcap > 0.f ? p.cap_k : p.scale_log2);
-  if (threadIdx.x < RN) {
-    const int r = threadIdx.x, gr = rt * RN + r;
-    float lse = INFINITY;                                  // rows that see nothing or do not exist weigh nothing
-    if (r < n) {
-      lse = p.a.lse[long(x.q0 + x.first + gr / G) * p.a.Hq + kvh * G + gr % G];
-      if (lse == -INFINITY) lse = INFINITY;
+    for (int o = 1; o < KH * 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float qs = kv8_scale_of(__uint_as_float(m << 16)), inv = kv8_inverse(qs);
+    if (ch == 0) {
+      const int gr = rt * RN + r;
+      float lse = INFINITY;                                // rows that see nothing or do not exist weigh nothing
+      if (r < n) {
+        lse = p.a.lse[long(x.q0 + x.first + gr / G) * p.a.Hq + kvh * G + gr % G];
+        if (lse == -INFINITY) lse = INFINITY;
+      }
+      head[r] = qs * (p.a.softcap > 0.f ? p.cap_k : p.scale_log2);
+      head[RN + r] = lse;
+      reinterpret_cast<int*>(head)[2 * RN + r] = r < n ? x.base + gr / G : -1;
     }
-    head[16 + r] = lse;
-    reinterpret_cast<int*>(head)[80 + r] = r < n ? x.base + gr / G : -1;
-  }
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int i = threadIdx.x + j * 256, r = i / (KH * 8), ch = i % (KH * 8);
     uint32_t hi4[4], lo4[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       hi4[k] = lo4[k] = 0u;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const uint32_t v = u[j][2 * k + e];
+        const uint32_t v = u[2 * k + e];
         const float a0 = __uint_as_float(v << 16) * inv, a1 = __uint_as_float(v & 0xffff0000u) * inv;
         uint32_t hh = e4m3x2(a0, a1);
         if ((v & 0x7f80u) == 0x7f80u) hh |= 0x7fu;
         if ((v & 0x7f800000u) == 0x7f800000u) hh |= 0x7f00u;
         const float2 f = __half22float2(e4m3x2_to_half2(hh));
         hi4[k] |= hh << (16 * e);
-        lo4[k] |= e4m3x2((a0 - f.x) * 16.f, (a1 - f.y) * 16.f) << (16 * e);
+        lo4[k] |= e4m3x2(a0 - f.x, a1 - f.y) << (16 * e);
       }
     }
-    uint8_t* dst = rec + HEAD + (ch / 8) * (NS * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+    uint8_t* dst = rec + HEAD + (ch / 8) * (RN * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
     *reinterpret_cast<uint4*>(dst) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
-    *reinterpret_cast<uint4*>(dst + RN * 128) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
+    *reinterpret_cast<uint4*>(dst + KH * RN * 128) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
   }
 }
 
 template <int KH>
 struct WCfg {
   static constexpr int K_BYTES = KH * 16384;              // two of them
-  static constexpr int R_BYTES = HEAD + KH * NS * 128, ST = KH == 1 ? 4 : 3;      // records in flight
+  static constexpr int R_BYTES = HEAD + 2 * KH * RN * 128, ST = KH == 1 ? 4 : 3;      // records in flight
   static constexpr int TAIL = 256;
   static constexpr int SMEM = 2 * K_BYTES + ST * R_BYTES + TAIL + 1024;           // two CTAs to an SM at KH = 1
 };
@@ -184,7 +178,7 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
     mbar_fence_init();
   }
   if (warp == 8) {
-    tmem_alloc(tmem_slot, 2 * NS);
+    tmem_alloc(tmem_slot, 2 * RN);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -222,7 +216,7 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
     }
   } else if (warp == 8) {
     if (lane == 0) {
-      constexpr uint32_t idesc = umma_idesc(128, NS, 0, 0, 0, 0);
+      constexpr uint32_t idesc = umma_idesc(128, RN, 0, 0, 0, 0);
       const uint64_t dk = umma_desc_k_sw128(smem_u32(k_s)), dq = umma_desc_k_sw128(smem_u32(r_s) + HEAD);
       bool ok = true;
       for (int i = 0; ok && i < rb - ra; ++i) {
@@ -235,10 +229,13 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
           tc_fence_after();
           const uint64_t da = dk + uint32_t(t) * (C::K_BYTES / 16);
 #pragma unroll
-          for (int h = 0; h < KH; ++h) {
+          for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f8(tmem + t * NS, da + (h * 1024 + k * 2), db + (h * (NS * 8) + k * 2), idesc, (h | k) ? 1u : 0u);
+            for (int h = 0; h < KH; ++h) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f8(tmem + t * RN, da + (h * 1024 + k * 2), db + ((e * KH + h) * (RN * 8) + k * 2), idesc, (e | h | k) ? 1u : 0u);
+            }
           }
           umma_commit(&s_full[t]);
         }
@@ -247,7 +244,7 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
     }
   } else {
     const int w = warp >> 2, tl = (warp & 3) * 32 + lane;
-    const uint32_t my_S = tmem + w * NS + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t my_S = tmem + w * RN + (uint32_t((warp & 3) * 32) << 16);
     const int tok = key0 + w * BKV + tl;
     float ks = 0.f, acc0 = 0.f, acc1 = 0.f;
     if (w < n_tiles && tok < x.ctx) {
@@ -268,28 +265,26 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
       if (w < n_tiles) {
         tc_fence_after();
         const float* head = reinterpret_cast<const float*>(r_s + st * C::R_BYTES);
-        const float mul = head[0] * ks;
         const int rt = ra + i, pos_a = x.base + rt * RN / G, pos_b = x.base + (min(x.rows, (rt + 1) * RN) - 1) / G;
         const int last = key0 + w * BKV + BKV - 1;
         const bool full = last < x.ctx && last <= pos_a && (p.a.window == 0 || last - BKV + 1 > pos_b - p.a.window);
 #pragma unroll 2
         for (int r0 = 0; r0 < RN; r0 += 16) {
-          uint32_t h16[16], l16[16];
-          tmem_ld16(my_S + r0, h16);
-          tmem_ld16(my_S + RN + r0, l16);
+          uint32_t sr[16];
+          tmem_ld16(my_S + r0, sr);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
-            const float4 lse = *reinterpret_cast<const float4*>(head + 16 + r0 + j);
-            const float ls[4] = {lse.x, lse.y, lse.z, lse.w};
+            const float4 f4 = *reinterpret_cast<const float4*>(head + r0 + j), l4 = *reinterpret_cast<const float4*>(head + RN + r0 + j);
+            const float fs[4] = {f4.x, f4.y, f4.z, f4.w}, ls[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float s = fmaf(__uint_as_float(l16[j + e]), 0.0625f, __uint_as_float(h16[j + e]));
+              const float raw = __uint_as_float(sr[j + e]), mul = fs[e] * ks;
               float y;
-              if constexpr (CAP) y = ex2(fmaf(softcap_r(s * mul, 1.f), p.scale_log2, 0.5f * p.scale_log2) - ls[e]);
-              else y = ex2(fmaf(s, mul, -ls[e]));
+              if constexpr (CAP) y = ex2(fmaf(softcap_r(raw * mul, 1.f), p.scale_log2, 0.5f * p.scale_log2) - ls[e]);
+              else y = ex2(fmaf(raw, mul, -ls[e]));
               if (!full) {
-                const int pos = reinterpret_cast<const int*>(head)[80 + r0 + j + e];
+                const int pos = reinterpret_cast<const int*>(head)[2 * RN + r0 + j + e];
                 if (tok > pos || tok >= x.ctx || (p.a.window > 0 && tok <= pos - p.a.window)) y = 0.f;
               }
               if (e & 1) acc1 += y;
@@ -308,7 +303,7 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
   __syncthreads();
   if (warp == 8) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * NS);
+    tmem_dealloc(tmem, 2 * RN);
   }
 }
 
@@ -372,7 +367,7 @@ int max_records(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int obser
 }  // namespace
 
 int64_t kv8_weights_scratch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int observe) {
-  return int64_t(s.n) * c.Hkv * max_records(c, s, a, observe) * (HEAD + (c.dk + 127) / 128 * NS * 128);
+  return int64_t(s.n) * c.Hkv * max_records(c, s, a, observe) * (HEAD + (c.dk + 127) / 128 * 2 * RN * 128);
 }
 
 int kv8_weights_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int observe, int tiles, void* scratch, float* w, long w_seq,
