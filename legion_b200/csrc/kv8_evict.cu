@@ -40,7 +40,7 @@ constexpr int HELD = 50 * 1024;        // images in a CTA's shared memory; those
 __global__ void __launch_bounds__(SELECT_THREADS) kv8_select_kernel(const EvictArgs p, int room) {
   namespace cg = cooperative_groups;
   extern __shared__ uint32_t held[];
-  __shared__ uint32_t hist[2048];
+  __shared__ __align__(16) uint32_t hist[2048];
   __shared__ uint32_t s_warp[32], s_gt[32], s_eq[32];
   __shared__ uint32_t s_digit, s_above, s_cta[2];
   griddep_wait();

@@ -182,6 +182,8 @@ class LmEngine(Engine):
         if kv8:
             if self.dp_world > 1 or getattr(model, "pipe", None) is not None or c.kv_rings:
                 raise ValueError("an 8-bit KV cache is not available with data-parallel attention, pipeline stages or window rings")
+            if dev.type == "cuda" and model.dtype != torch.bfloat16:
+                raise ValueError("an 8-bit KV cache is for bfloat16 models on a GPU")
             c.kv_swap_gib = 0.0                 # preempted sequences are recomputed, evicted prefixes dropped
             c.prefix_host_gib = 0.0
         if c.kv_rings and "swa" in self.mcfg.layer_kinds and self.mcfg.sliding_window > 0:

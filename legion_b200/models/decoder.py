@@ -93,9 +93,9 @@ class KvCache:
         with a scale per block and head (``ops.Kv8Cache``, the same object under ``k`` and ``v``)."""
         self.page, self.n_blocks, self.kv8 = page, n_blocks, kv8
         if kv8 and (cfg.layers is not None or cfg.kv_lora > 0 or cfg.sandwich_norm or cfg.block_form or cfg.hyper_streams > 1
-                    or "mla" in cfg.layer_kinds or cfg.head_dim % 16 or ring_blocks):
+                    or "mla" in cfg.layer_kinds or cfg.head_dim % 16 or cfg.head_dim > 256 or page not in (8, 16, 32, 64) or ring_blocks):
             raise ValueError("an 8-bit KV cache is for models whose attention layers keep plain keys and values of 16, 32, .. 256 "
-                             "columns, without window rings")
+                             "columns, in blocks of 8 to 64 tokens, without window rings")
         self.ring_blocks = ring_blocks
         self._kinds = tuple(cfg.layer_kinds)
         self.k: Dict[int, torch.Tensor] = {}

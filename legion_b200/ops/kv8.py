@@ -101,7 +101,8 @@ def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: in
 
     ``weights`` float32 [sequences, kv heads, >= longest context]: every key's softmax weight, summed over the query heads that
     share its head and over the sequence's last ``observe`` rows (0: all of the call), is added to its sum: what ``kv8_evict`` goes
-    by. The sums do not depend on the order of anything but the rows."""
+    by. The sums do not depend on the order of anything but the rows. A decode call with sums takes 4 bytes of scratch per row, head
+    and key up to ``max_ctx``."""
     if not q.is_cuda:
         _check(cache, "kv8_attention")
         if q.dim() != 3 or q.shape[2] != cache.k.shape[3] or q.shape[1] % cache.k.shape[1]:

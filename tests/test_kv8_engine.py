@@ -97,6 +97,8 @@ def test_copy_blocks():
 def test_refusals():
     with pytest.raises(ValueError, match="8-bit"):
         KvCache(tiny_mla_moe(), 4, 16, "cpu", torch.float32, kv8=True)
+    with pytest.raises(ValueError, match="8-bit"):
+        KvCache(tiny_dense(), 4, 128, "cpu", torch.float32, kv8=True)
     with pytest.raises(ValueError, match="kv_dtype"):
         engine("dense", kv_dtype="int3")
     with pytest.raises(ValueError, match="rings"):
