@@ -235,58 +235,67 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   const uint32_t tmem = *tmem_slot;
   auto fail = [&](int code) { *abort_flag = 1; atomicCAS(p.s.status, 0, code | SITE_PREFILL_ATTN); return false; };
 
-  // Queries, by the softmax and the value warps, a row at a time: a power of two, two e4m3 terms. Not finite: a NaN code.
+  // Queries, by the softmax and the value warps, a row at a time: a power of two, two e4m3 terms. Not finite: a NaN code. Eight rows
+  // are fetched at once: a fetch behind another row's stores waits for them, and 22 rows in a chain took 12 us.
   if (wg <= RT) {
-    const int dims = KH * 4;                            // of a lane
-#pragma unroll 4
-    for (int r = warp; r < RT * 128; r += (RT + 1) * 4) {
-      const int gr = row0 + r;
-      uint32_t u[KH * 2];
+    constexpr int DIMS = KH * 4, NW = (RT + 1) * 4, ROWS = 8;      // columns of a lane, warps, rows in flight
+    const int d = lane * DIMS, ch = d / 16;
+#pragma unroll 1
+    for (int r0 = warp; r0 < RT * 128; r0 += NW * ROWS) {
+      uint32_t u[ROWS][KH * 2];
 #pragma unroll
-      for (int k = 0; k < KH * 2; ++k) u[k] = 0u;
-      if (r < rows && lane * dims < c.dk) {
-        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + (long(q0) + gr / G) * p.a.q_tok + (kvh * G + gr % G) * p.a.q_head +
-                                   lane * dims;
-        if ((reinterpret_cast<uintptr_t>(src) & (KH * 8 - 1)) == 0) {
-          if (KH == 1) *reinterpret_cast<uint2*>(u) = *reinterpret_cast<const uint2*>(src);
-          else *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(src);
-        } else {
-          const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+      for (int i = 0; i < ROWS; ++i) {
+        const int r = r0 + i * NW, gr = row0 + r;
 #pragma unroll
-          for (int k = 0; k < KH * 2; ++k) u[k] = h[2 * k] | uint32_t(h[2 * k + 1]) << 16;
+        for (int k = 0; k < KH * 2; ++k) u[i][k] = 0u;
+        if (r < rows && d < c.dk) {
+          const int tok = gr / G;
+          const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + (long(q0) + tok) * p.a.q_tok + (kvh * G + gr - tok * G) * p.a.q_head + d;
+          if ((reinterpret_cast<uintptr_t>(src) & (KH * 8 - 1)) == 0) {
+            if (KH == 1) *reinterpret_cast<uint2*>(u[i]) = *reinterpret_cast<const uint2*>(src);
+            else *reinterpret_cast<uint4*>(u[i]) = *reinterpret_cast<const uint4*>(src);
+          } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+            for (int k = 0; k < KH * 2; ++k) u[i][k] = h[2 * k] | uint32_t(h[2 * k + 1]) << 16;
+          }
         }
       }
-      uint32_t m = 0;
 #pragma unroll
-      for (int k = 0; k < KH * 2; ++k) {
-        const uint32_t lo = u[k] & 0x7fffu, hi = (u[k] >> 16) & 0x7fffu;
-        m = max(m, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
-      }
-      m = __reduce_max_sync(0xffffffffu, m);
-      const float qs = kv8_scale_of(__uint_as_float(m << 16)), inv = kv8_inverse(qs);
-      if (lane == 0) s_q[r] = qs * (CAP ? p.cap_k : p.scale_log2);
-      uint32_t hi4[KH], lo4[KH];
+      for (int i = 0; i < ROWS; ++i) {
+        const int r = r0 + i * NW;
+        if (r >= RT * 128) break;
+        uint32_t m = 0;
 #pragma unroll
-      for (int k = 0; k < KH * 2; ++k) {
-        const float a0 = __uint_as_float(u[k] << 16) * inv, a1 = __uint_as_float(u[k] & 0xffff0000u) * inv;
-        uint32_t hh = e4m3x2(a0, a1);
-        if ((u[k] & 0x7f80u) == 0x7f80u) hh |= 0x7fu;
-        if ((u[k] & 0x7f800000u) == 0x7f800000u) hh |= 0x7f00u;
-        const float2 f = __half22float2(e4m3x2_to_half2(hh));
-        // the remainder in the units of the first term: its lower end, 2^-10 of a largest code of 128 or more, is 2^-17 of the row's
-        // largest value; bf16 values that small have a step of 2^-9 of themselves
-        const uint32_t ll = e4m3x2(a0 - f.x, a1 - f.y);
-        if (k & 1) { hi4[k / 2] |= hh << 16; lo4[k / 2] |= ll << 16; }
-        else { hi4[k / 2] = hh; lo4[k / 2] = ll; }
-      }
-      const int d = lane * dims, ch = d / 16;
-      uint8_t* dst = q_s + ((r / 128) * 2 * KH + ch / 8) * 16384 + (r % 128) * 128 + (((ch & 7) ^ (r & 7)) << 4) + d % 16;
-      if (KH == 1) {
-        *reinterpret_cast<uint32_t*>(dst) = hi4[0];
-        *reinterpret_cast<uint32_t*>(dst + KH * 16384) = lo4[0];
-      } else {
-        *reinterpret_cast<uint2*>(dst) = make_uint2(hi4[0], hi4[KH - 1]);
-        *reinterpret_cast<uint2*>(dst + KH * 16384) = make_uint2(lo4[0], lo4[KH - 1]);
+        for (int k = 0; k < KH * 2; ++k) {
+          const uint32_t lo = u[i][k] & 0x7fffu, hi = (u[i][k] >> 16) & 0x7fffu;
+          m = max(m, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+        }
+        m = __reduce_max_sync(0xffffffffu, m);
+        const float qs = kv8_scale_of(__uint_as_float(m << 16)), inv = kv8_inverse(qs);
+        if (lane == 0) s_q[r] = qs * (CAP ? p.cap_k : p.scale_log2);
+        uint32_t hi4[KH], lo4[KH];
+#pragma unroll
+        for (int k = 0; k < KH * 2; ++k) {
+          const float a0 = __uint_as_float(u[i][k] << 16) * inv, a1 = __uint_as_float(u[i][k] & 0xffff0000u) * inv;
+          uint32_t hh = e4m3x2(a0, a1);
+          if ((u[i][k] & 0x7f80u) == 0x7f80u) hh |= 0x7fu;
+          if ((u[i][k] & 0x7f800000u) == 0x7f800000u) hh |= 0x7f00u;
+          const float2 f = __half22float2(e4m3x2_to_half2(hh));
+          // the remainder in the units of the first term: its lower end, 2^-10 of a largest code of 128 or more, is 2^-17 of the
+          // row's largest value; bf16 values that small have a step of 2^-9 of themselves
+          const uint32_t ll = e4m3x2(a0 - f.x, a1 - f.y);
+          if (k & 1) { hi4[k / 2] |= hh << 16; lo4[k / 2] |= ll << 16; }
+          else { hi4[k / 2] = hh; lo4[k / 2] = ll; }
+        }
+        uint8_t* dst = q_s + ((r / 128) * 2 * KH + ch / 8) * 16384 + (r % 128) * 128 + (((ch & 7) ^ (r & 7)) << 4) + d % 16;
+        if (KH == 1) {
+          *reinterpret_cast<uint32_t*>(dst) = hi4[0];
+          *reinterpret_cast<uint32_t*>(dst + KH * 16384) = lo4[0];
+        } else {
+          *reinterpret_cast<uint2*>(dst) = make_uint2(hi4[0], hi4[KH - 1]);
+          *reinterpret_cast<uint2*>(dst + KH * 16384) = make_uint2(lo4[0], lo4[KH - 1]);
+        }
       }
     }
     fence_proxy_async_smem();
