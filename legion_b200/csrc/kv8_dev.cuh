@@ -41,7 +41,8 @@ __device__ __forceinline__ float kv8_scale_of(float amax) {
   const int e = int(__float_as_uint(amax) >> 23) - 127;
   return __uint_as_float(uint32_t(max(e - 7, -60) + 127) << 23);
 }
-__device__ __forceinline__ float kv8_inverse(float scale) { return scale > 0.f ? 1.f / scale : 0.f; }
+// 1 / scale of a power of two (2^-60 .. 2^120), 0 for 0: the exponent turned round, without a division's code
+__device__ __forceinline__ float kv8_inverse(float scale) { return scale > 0.f ? __uint_as_float(0x7f000000u - __float_as_uint(scale)) : 0.f; }
 __device__ __forceinline__ int kv8_log2(float scale) {
   return scale > 0.f ? max(-120, min(120, int(__float_as_uint(scale) >> 23) - 127)) : 0;
 }
