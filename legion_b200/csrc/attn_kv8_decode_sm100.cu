@@ -21,9 +21,13 @@
 // Two softmax warpgroups (warps 0..3 and 4..7; thread = key of the tile, later output column) take alternate tiles, each a
 // stream of its own with its P and O^T; they meet in shared memory at the end of a piece. Warp 8: the scores' MMAs, four tiles ahead
 // of their softmax (a wait for a phase of a stage's barrier cannot miss it: the stage's next scores stand behind P of this tile,
-// the stage's next P V behind P of the tile that waits). Warps 9, 12: TMA of keys and of values through the block
-// table into as many stages as fit (six of 32 KB for heads of 128), and the tiles' scales. Warp 10: the next piece's queries. Warp 11: P V. Code that runs
-// once a piece or rarely is kept short: unrolled over the heads it was fetched at 6000 clocks a piece.
+// the stage's next P V behind P of the tile that waits). Warps 9, 12: TMA of keys and of values through the block table into as
+// many stages as fit (six of 32 KB for heads of 128), and the tiles' scales. Warp 10: the next piece's queries. Warp 11: P V. Code
+// that runs once a piece or rarely is kept short: unrolled over the heads it was fetched at 6000 clocks a piece.
+//
+// 16 sequences of 8192 tokens, 32 / 4 heads of 128: 37.6 us = 3.6 TB/s with the join, 0.55 of the measured copy rate. In its steady
+// state a tile takes an SM 1200 to 1370 clocks, which is the memory's rate; the rest is the launch's beginning (lengths, table,
+// first keys: dependent reads, and instructions fetched behind them) and its end.
 #include "kv8_dev.cuh"
 #include "tmap.cuh"
 

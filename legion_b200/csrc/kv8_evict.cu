@@ -7,7 +7,8 @@
 // that stay in any case are outside the search. It is kept small: a launch fetches its code anew. (4 sequences of 32K tokens and 4
 // heads: one CTA each 45 us, weights in registers by unrolled code 75, clusters of eight 63: half of them wait for the others.)
 // kv8_move_kernel, one CTA per (block of the result, kv head, keys or values): gathers its rows. The block's scale is the largest of
-// those that its rows come from, so a code moves by a power of two: bit for bit where the scales agree.
+// those that its rows come from, so a code moves by a power of two: bit for bit where the scales agree. 4 sequences of 32K tokens to
+// 4096, 4 heads of 128: selection 25 us (shared-memory atomics), moving 12 us.
 #include <cooperative_groups.h>
 
 #include "kv8_dev.cuh"
