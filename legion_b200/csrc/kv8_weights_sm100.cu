@@ -10,7 +10,10 @@
 // S^T[128 keys, 64 rows] = K . Q^T on tcgen05, with the terms, scales and order of the attention, whose sums its scores have to be
 // bit for bit: the tensor cores cut off what does not fit a sum, and scores summed in another order gave weights 10^-6 too large.
 // A thread has a key and adds up its columns over all records, so nothing crosses threads and the result does not depend on any
-// order but the rows' own. 64 exponentials per key and record bound it: 64 rows of 32 heads over 16K keys take 25 us.
+// order but the rows' own. Two score tiles are made ahead of their use. 64 exponentials per key and record
+// and the records' traffic bound it: 64 rows of 32 heads over 16K keys add 30 us to the call, all 1024 rows 295 (a mask branch per
+// score instead of per record and one score tile: 57 and 510).
+#include <type_traits>
 #include "kv8_dev.cuh"
 #include "tmap.cuh"
 
@@ -141,9 +144,9 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
   uint64_t* k_full = bars;         // [2]
   uint64_t* r_full = bars + 2;     // [4]
   uint64_t* r_empty = bars + 6;    // [4]
-  uint64_t* s_full = bars + 10;    // [2]
-  uint64_t* s_empty = bars + 12;   // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+  uint64_t* s_full = bars + 10;    // [2 tiles][2 buffers]
+  uint64_t* s_empty = bars + 14;   // [2][2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const Kv8Cache& c = p.c;
@@ -165,8 +168,8 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
   if (ra >= rb) return;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&k_full[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&k_full[i], 1);
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&s_empty[i], 128);
     }
@@ -178,7 +181,7 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
     mbar_fence_init();
   }
   if (warp == 8) {
-    tmem_alloc(tmem_slot, 2 * RN);
+    tmem_alloc(tmem_slot, 4 * RN);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -224,7 +227,9 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
         if (!mbar_wait(&r_full[st], (i / ST) & 1, abort_flag)) { fail(ST_TIMEOUT_FULL); break; }
         const uint64_t db = dq + uint32_t(st) * (C::R_BYTES / 16);
         for (int t = 0; ok && t < n_tiles; ++t) {
-          ok = (i == 0 ? mbar_wait(&k_full[t], 0, abort_flag) : mbar_wait(&s_empty[t], (i - 1) & 1, abort_flag)) || fail(ST_TIMEOUT_TMEM_EMPTY);
+          const int sb = t * 2 + (i & 1);
+          ok = (i == 0 ? mbar_wait(&k_full[t], 0, abort_flag) : i < 2 || mbar_wait(&s_empty[sb], ((i >> 1) - 1) & 1, abort_flag)) ||
+               fail(ST_TIMEOUT_TMEM_EMPTY);
           if (!ok) break;
           tc_fence_after();
           const uint64_t da = dk + uint32_t(t) * (C::K_BYTES / 16);
@@ -234,17 +239,17 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
             for (int h = 0; h < KH; ++h) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                umma_f8(tmem + t * RN, da + (h * 1024 + k * 2), db + ((e * KH + h) * (RN * 8) + k * 2), idesc, (e | h | k) ? 1u : 0u);
+                umma_f8(tmem + sb * RN, da + (h * 1024 + k * 2), db + ((e * KH + h) * (RN * 8) + k * 2), idesc, (e | h | k) ? 1u : 0u);
             }
           }
-          umma_commit(&s_full[t]);
+          umma_commit(&s_full[sb]);
         }
         if (ok) umma_commit(&r_empty[st]);
       }
     }
   } else {
     const int w = warp >> 2, tl = (warp & 3) * 32 + lane;
-    const uint32_t my_S = tmem + w * RN + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t my_lane = uint32_t((warp & 3) * 32) << 16;
     const int tok = key0 + w * BKV + tl;
     float ks = 0.f, acc0 = 0.f, acc1 = 0.f;
     if (w < n_tiles && tok < x.ctx) {
@@ -257,43 +262,48 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
       const int st = i % ST;
       // the record's head (its codes go to the MMA), then the scores made from it. (A warpgroup without a tile keeps step, too.)
       ok = __all_sync(0xffffffffu, mbar_wait(&r_full[st], (i / ST) & 1, abort_flag)) &&
-           (w >= n_tiles || __all_sync(0xffffffffu, mbar_wait(&s_full[w], i & 1, abort_flag)));
+           (w >= n_tiles || __all_sync(0xffffffffu, mbar_wait(&s_full[w * 2 + (i & 1)], (i >> 1) & 1, abort_flag)));
       if (!ok) {
         if (lane == 0) fail(ST_TIMEOUT_TMEM_FULL);
         break;
       }
       if (w < n_tiles) {
         tc_fence_after();
+        const uint32_t my_S = tmem + (w * 2 + (i & 1)) * RN + my_lane;
         const float* head = reinterpret_cast<const float*>(r_s + st * C::R_BYTES);
         const int rt = ra + i, pos_a = x.base + rt * RN / G, pos_b = x.base + (min(x.rows, (rt + 1) * RN) - 1) / G;
         const int last = key0 + w * BKV + BKV - 1;
         const bool full = last < x.ctx && last <= pos_a && (p.a.window == 0 || last - BKV + 1 > pos_b - p.a.window);
+        auto add_up = [&](auto masked) {
 #pragma unroll 2
-        for (int r0 = 0; r0 < RN; r0 += 16) {
-          uint32_t sr[16];
-          tmem_ld16(my_S + r0, sr);
-          tmem_ld_wait();
+          for (int r0 = 0; r0 < RN; r0 += 16) {
+            uint32_t sr[16];
+            tmem_ld16(my_S + r0, sr);
+            tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            const float4 f4 = *reinterpret_cast<const float4*>(head + r0 + j), l4 = *reinterpret_cast<const float4*>(head + RN + r0 + j);
-            const float fs[4] = {f4.x, f4.y, f4.z, f4.w}, ls[4] = {l4.x, l4.y, l4.z, l4.w};
+            for (int j = 0; j < 16; j += 4) {
+              const float4 f4 = *reinterpret_cast<const float4*>(head + r0 + j), l4 = *reinterpret_cast<const float4*>(head + RN + r0 + j);
+              const float fs[4] = {f4.x, f4.y, f4.z, f4.w}, ls[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float raw = __uint_as_float(sr[j + e]), mul = fs[e] * ks;
-              float y;
-              if constexpr (CAP) y = ex2(fmaf(softcap_r(raw * mul, 1.f), p.scale_log2, 0.5f * p.scale_log2) - ls[e]);
-              else y = ex2(fmaf(raw, mul, -ls[e]));
-              if (!full) {
-                const int pos = reinterpret_cast<const int*>(head)[2 * RN + r0 + j + e];
-                if (tok > pos || tok >= x.ctx || (p.a.window > 0 && tok <= pos - p.a.window)) y = 0.f;
+              for (int e = 0; e < 4; ++e) {
+                const float raw = __uint_as_float(sr[j + e]), mul = fs[e] * ks;
+                float y;
+                if constexpr (CAP) y = ex2(fmaf(softcap_r(raw * mul, 1.f), p.scale_log2, 0.5f * p.scale_log2) - ls[e]);
+                else y = ex2(fmaf(raw, mul, -ls[e]));
+                if constexpr (decltype(masked)::value) {
+                  const int pos = reinterpret_cast<const int*>(head)[2 * RN + r0 + j + e];
+                  if (tok > pos || tok >= x.ctx || (p.a.window > 0 && tok <= pos - p.a.window)) y = 0.f;
+                }
+                if (e & 1) acc1 += y;
+                else acc0 += y;
               }
-              if (e & 1) acc1 += y;
-              else acc0 += y;
             }
           }
-        }
+        };
+        if (full) add_up(std::false_type{});        // (a branch per record, not per score)
+        else add_up(std::true_type{});
         tc_fence_before();
-        mbar_arrive(&s_empty[w]);
+        mbar_arrive(&s_empty[w * 2 + (i & 1)]);
       }
       if (lane == 0) mbar_arrive(&r_empty[st]);
     }
@@ -303,7 +313,7 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
   __syncthreads();
   if (warp == 8) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * RN);
+    tmem_dealloc(tmem, 4 * RN);
   }
 }
 
