@@ -2,7 +2,9 @@
 // exp(score - lse), with the log-sum-exp of every row and head from the attention itself.
 //
 // Decode: the attention kernel leaves its scores (4 bytes a head and key, an eighth of the keys' own bytes at 4 to 8 heads of 128
-// per kv head, where scores made anew would read all keys again), and kv8_score_sums_kernel adds them up, a thread per key.
+// per kv head, where scores made anew would read all keys again), and kv8_score_sums_kernel adds them up,
+// four keys to a thread so that their loads fly together (64 sequences of 750 to 2250 keys: 8 us alone, 17 with one key and a
+// shared copy of the log-sum-exps).
 //
 // Rows of a prompt: the scores once more. kv8_queries_kernel packs the rows that count, 64 (token, head) rows of a kv head to a
 // record: their two e4m3 terms in the layout that the MMA reads, powers of two, log-sum-exps and positions. kv8_weights_kernel,
@@ -21,6 +23,7 @@ namespace lb {
 namespace {
 
 constexpr int RN = 64, BKV = 128;
+constexpr int SUM_THREADS = 128, SUM_KEYS = 4;      // of kv8_score_sums_kernel: keys of a thread lie SUM_THREADS apart
 constexpr int HEAD = 1024;               // of a record: powers of two [64], log-sum-exps [64], positions [64]; behind it the first, then the second terms
 
 struct WeightArgs {
@@ -318,36 +321,43 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
 }
 
 // scores [T][Hq][span] of a decode call, from the first visible tile on
-__global__ void __launch_bounds__(256) kv8_score_sums_kernel(const WeightArgs p, const float* scores, int span) {
-  __shared__ float s_lse[256];
+__global__ void __launch_bounds__(SUM_THREADS) kv8_score_sums_kernel(const WeightArgs p, const float* scores, int span) {
   griddep_wait();
   griddep_launch();
   const int G = p.a.Hq / p.c.Hkv, kvh = blockIdx.y, seq = blockIdx.z;
-  const int row = p.s.cu[seq];
-  if (row < 0 || row >= p.s.T || p.s.cu[seq + 1] != row + 1) return;
-  const int ctx = int(min(long(max(p.s.ctx[seq], 0)), long(p.s.width) * p.c.page));
+  const int row = p.s.cu[seq], next = p.s.cu[seq + 1], len = p.s.ctx[seq];
+  if (row < 0 || row >= p.s.T || next != row + 1) return;
+  const int ctx = int(min(long(max(len, 0)), long(p.s.width) * p.c.page));
   const int start = (p.a.window > 0 && ctx > p.a.window) ? ctx - p.a.window : 0, base = start / BKV * BKV;
   if (ctx > p.w_keys || ctx - base > span) {
     if (threadIdx.x == 0) atomicCAS(p.s.status, 0, ST_BAD_ARGS);
     return;
   }
-  if (base + int(blockIdx.x) * 256 >= ctx) return;
-  const int tok = base + blockIdx.x * 256 + threadIdx.x;
+  const int first = base + int(blockIdx.x) * (SUM_THREADS * SUM_KEYS);
+  if (first >= ctx) return;
+  const int tok = first + threadIdx.x;
   const float* s = scores + (long(row) * p.a.Hq + kvh * G) * span + (tok - base);
-  float acc = 0.f;
-  for (int g0 = 0; g0 < G; g0 += 256) {
-    __syncthreads();
-    if (g0 + int(threadIdx.x) < G) {
-      const float l = p.a.lse[long(row) * p.a.Hq + kvh * G + g0 + threadIdx.x];
-      s_lse[threadIdx.x] = l == -INFINITY ? INFINITY : l;
-    }
-    __syncthreads();
-    if (tok >= start && tok < ctx) {
-#pragma unroll 8
-      for (int g = 0; g < min(256, G - g0); ++g) acc += ex2(s[long(g0 + g) * span] - s_lse[g]);
-    }
+  const float* lse = p.a.lse + long(row) * p.a.Hq + kvh * G;
+  float* w = p.w + seq * p.w_seq + kvh * p.w_head + tok;
+  bool in[SUM_KEYS];
+  float acc[SUM_KEYS], was[SUM_KEYS];
+#pragma unroll
+  for (int k = 0; k < SUM_KEYS; ++k) {
+    const int t = tok + k * SUM_THREADS;
+    in[k] = t >= start && t < ctx;
+    acc[k] = 0.f;
+    was[k] = in[k] ? w[k * SUM_THREADS] : 0.f;
   }
-  if (tok >= start && tok < ctx) p.w[seq * p.w_seq + kvh * p.w_head + tok] += acc;
+#pragma unroll 4
+  for (int g = 0; g < G; ++g) {
+    const float l = lse[g], sub = l == -INFINITY ? INFINITY : l;
+#pragma unroll
+    for (int k = 0; k < SUM_KEYS; ++k)
+      if (in[k]) acc[k] += ex2(s[long(g) * span + k * SUM_THREADS] - sub);
+  }
+#pragma unroll
+  for (int k = 0; k < SUM_KEYS; ++k)
+    if (in[k]) w[k * SUM_THREADS] = was[k] + acc[k];
 }
 
 WeightArgs make(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, float* w, long w_seq, long w_head, int w_keys) {
@@ -403,7 +413,8 @@ int kv8_score_sums_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a,
                           long w_head, int w_keys, cudaStream_t st) {
   if (s.n <= 0 || s.T <= 0) return 0;
   const WeightArgs p = make(c, s, a, w, w_seq, w_head, w_keys);
-  const cudaError_t e = launch_pdl(kv8_score_sums_kernel, dim3((span + 255) / 256, c.Hkv, s.n), dim3(256), 0, st, p, scores, span);
+  const cudaError_t e = launch_pdl(kv8_score_sums_kernel, dim3((span + SUM_THREADS * SUM_KEYS - 1) / (SUM_THREADS * SUM_KEYS), c.Hkv, s.n),
+                                   dim3(SUM_THREADS), 0, st, p, scores, span);
   if (e != cudaSuccess) kv8_set_error(cudaGetErrorString(e));
   return e != cudaSuccess;
 }
