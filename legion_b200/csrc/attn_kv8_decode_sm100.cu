@@ -10,7 +10,7 @@
 //     turns back into a half by a byte move and the remainder is one exact half subtraction.
 // Scales never touch the codes: a key's scale multiplies its score, and a value's scale 2^e joins the exponent, z = s + e, so
 // that the running reference is the largest weight a code can get, P stays in the range of a half whatever the scales are, and
-// the denominator adds exp(z) 2^-e.
+// the denominator adds exp(z) 2^-e (in 32 bits: a weight of 2^-37 next to a value scale 2^100 times its own).
 //
 // One CTA per SM, and all of them share the batch's tiles evenly: the tiles of all (sequence, kv head) groups in a row, cut into
 // equal stretches, whatever the lengths are. A stretch ends one group, has some whole ones and begins another; a CTA goes through

@@ -1,0 +1,76 @@
+"""The 8-bit key/value cache where it meets the unusual: blocks of zeros, scattered NaN values, lengths beyond the block table, ragged
+batches with sums, long sums, malformed calls. Against float64 forms, with the tolerances that ``test_kv8`` derives."""
+import math
+
+import pytest
+import torch
+
+from legion_b200 import ops
+from test_kv8 import NAN, WHERE, attend, cum, filled, gen, gpu, i32, near, on, randn, status, tables
+
+
+def call(device, q, cache, table, lens, new, scale, **more):
+    more = {k: v.to(device) if isinstance(v, torch.Tensor) and k == "sink" else v for k, v in more.items()}
+    return ops.kv8_attention(q.to(device), cache, i32(table, device), i32(lens, device), i32(cum(new), device), max(new), scale, **more)
+
+
+def holding(k, v, page, device, seed=0):
+    """A cache with one sequence of these rows, its table."""
+    n, heads = k.shape[:2]
+    table, blocks = tables([n], page, seed)
+    cache = ops.Kv8Cache.empty(blocks, page, heads, k.shape[2], v.shape[2])
+    ops.kv8_append(cache, k.bfloat16(), v.bfloat16(), i32(table), i32([n]), i32([0, n]), n)
+    return on(cache, device), table
+
+
+# ----------------------------------------------------------------------------------------------- value blocks of zeros
+def near_sums(got, start, weight, off):
+    want, tol = weight.sum(2), off.sum(2)
+    assert bool(((got.cpu().double() - start.double() - want).abs() <= tol + 2.0 ** -23 * (start.double() + want)).all())
+
+
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("size", [0, -13, -20, -24, -50])
+@pytest.mark.parametrize("form", ["plain", "sink"])
+def test_zero_values_beside_small_ones(device, new, size, form):
+    """A block whose values are all zero has the scale 0. It adds to the denominator and takes nothing from the bits of the others,
+    however small they are."""
+    n, heads, kv, D = 256, 8, 2, 64
+    v = randn(n, kv, D, seed=2) * 2.0 ** size
+    v[32:48] = 0
+    cache, table = holding(randn(n, kv, D, seed=1), v, 16, device)
+    assert not bool(cache.v_scale[table[0][2]].any())
+    q, more = randn(new, heads, D, seed=3).bfloat16(), {"sink": randn(heads, seed=4)} if form == "sink" else {}
+    want, tol, weight, off = attend(q, cache, table, [n], [new], 0.125, **more)
+    start = torch.rand(1, kv, n, generator=gen(5))
+    w = start.clone().to(device)
+    near(call(device, q, cache, table, [n], [new], 0.125, weights=w, **more), want, tol)
+    near_sums(w[0], start[0], weight[0], off[0])
+    assert status(device) == 0
+
+
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("sink", [False, True])
+def test_nothing_but_zero_values(device, new, sink):
+    n, heads, kv, D = 300, 4, 2, 32
+    cache, table = holding(randn(n, kv, D, seed=1), torch.zeros(n, kv, D), 32, device)
+    q, more = randn(new, heads, D, seed=3).bfloat16(), {"sink": randn(heads, seed=4)} if sink else {}
+    _, _, weight, off = attend(q, cache, table, [n], [new], 0.2, **more)
+    w = torch.zeros(1, kv, n, device=device)
+    assert not bool(call(device, q, cache, table, [n], [new], 0.2, weights=w, **more).any())
+    near_sums(w[0], torch.zeros(kv, n), weight[0], off[0])
+    assert status(device) == 0
+
+
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("sharp", [1.0, 30.0])
+def test_prompt_far_apart_scales(device, sharp):
+    """Rows of a prompt over blocks whose values differ by 2^40."""
+    n, new = 300, 50
+    v = randn(n, 1, 64, seed=2) * torch.exp2(torch.linspace(-30, 10, n).round())[torch.randperm(n, generator=gen(3))].view(n, 1, 1)
+    cache, table = holding(randn(n, 1, 64, seed=1), v, 16, device)
+    q = randn(new, 8, 64, seed=5).mul(sharp).bfloat16()
+    want, tol, _, _ = attend(q, cache, table, [n], [new], 0.125)
+    near(call(device, q, cache, table, [n], [new], 0.125), want, tol)
