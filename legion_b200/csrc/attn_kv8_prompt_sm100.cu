@@ -45,7 +45,7 @@ struct PCfg {
   // registers of a softmax thread and of the others: together what the launch has (512 x 128 or 384 x 168)
   static constexpr int REGS_ROW = RT == 2 ? 184 : 232, REGS_REST = RT == 2 ? 72 : 136;
   static_assert(RT * 128 * REGS_ROW + 256 * REGS_REST <= (RT == 2 ? 512 * 128 : 384 * 168), "registers");
-  static constexpr int TAIL = 1280 + RT * 512;
+  static constexpr int TAIL = 1280 + RT * 512 + MT * 512;
   static constexpr int SMEM = Q_BYTES + KS * K_BYTES + V8S * V8_BYTES + V16S * V16_BYTES + TAIL;
   static constexpr int O_COL = 256;      // score buffers at 0 and 128
   static_assert(SMEM <= 227 * 1024 && O_COL + RT * MT * 128 <= 512, "sizes");
@@ -152,6 +152,33 @@ __device__ __forceinline__ void row_of_tile(uint32_t my_S, const float4* sc, flo
   top = fmaxf(mx0, mx1);
 }
 
+// Columns d .. d + 31 in which a key of [lo, hi) has a NaN value, a bit each. `first`: the first such key of each column. Where it
+// lies in front of the row's window, the codes of the window are looked through.
+__device__ __forceinline__ uint32_t nan_columns(const Kv8Cache& c, const int* table, int kvh, int d, const int* first, int lo, int hi) {
+  uint32_t seen = 0, look = 0;
+#pragma unroll 1
+  for (int j = 0; j < 32; ++j) {
+    const int f = first[j];
+    if (f < lo) look |= 1u << j;
+    else if (f < hi) seen |= 1u << j;
+  }
+#pragma unroll 1
+  for (int tok = lo; tok < hi && look; ++tok) {
+    const int blk = table[tok / c.page];
+    if (unsigned(blk) >= unsigned(c.n_blocks)) continue;
+    const uint8_t* src = c.v + ((long(blk) * c.Hkv + kvh) * c.page + tok % c.page) * c.dv + d;
+    uint32_t found = 0;
+#pragma unroll 1
+    for (int k = 0; k < 32 && d + k < c.dv; k += 4) {
+      const uint32_t m = (*reinterpret_cast<const uint32_t*>(src + k) & 0x7f7f7f7fu) + 0x01010101u;
+      found |= ((m >> 7 & 1u) | (m >> 14 & 2u) | (m >> 21 & 4u) | (m >> 28 & 8u)) << k;
+    }
+    seen |= found & look;
+    look &= ~found;
+  }
+  return seen;
+}
+
 template <int KH, int MT, bool CAP, bool WIDE>
 __global__ void __launch_bounds__(PCfg<KH, MT>::THREADS, 1)
 kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PromptArgs p) {
@@ -180,10 +207,10 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   uint64_t* sc_full = bars + 19;    // [4]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* s_nan = reinterpret_cast<int*>(bars + 24);       // first and last key with a NaN value, then a bit per column [8]
+  int* s_nan = reinterpret_cast<int*>(bars + 24);       // first and last key with a NaN value
   float4* s_sc = reinterpret_cast<float4*>(bars + 32);  // [4][16]: key scale, log2 of the value scale 2^e, 2^-e, per 8 keys
-
   float* s_q = reinterpret_cast<float*>(bars + 160);    // [RT * 128]: a row's power of two times the score scale
+  int* s_first = reinterpret_cast<int*>(s_q + RT * 128);      // [MT * 128]: a column's first key with a NaN value
 
   const Kv8Cache& c = p.c;
   const int G = p.a.Hq / c.Hkv;
@@ -226,9 +253,9 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     *abort_flag = 0;
     s_nan[0] = 0x7fffffff;
     s_nan[1] = -1;
-    for (int i = 0; i < 8; ++i) s_nan[2 + i] = 0;
     mbar_fence_init();
   }
+  for (int i = threadIdx.x; i < MT * 128; i += C::THREADS) s_first[i] = 0x7fffffff;
   if (warp == (RT + 1) * 4) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -436,14 +463,15 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
         for (int j = 0; j < 32; ++j) any |= (x[j] & 0x7f7f7f7fu) + 0x01010101u;
         if (any & 0x80808080u) {
-          // NaN codes: noted (rows that see one become NaN at the end), and not multiplied with the zeros of rows that do not
+          // NaN codes: noted (at the end, rows become NaN in the columns of those they see), and not multiplied with the zeros of
+          // rows that do not
           atomicMin(&s_nan[0], tok);
           atomicMax(&s_nan[1], tok);
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             for (int e = 0; e < 4; ++e) {
               if (((x[j] >> (8 * e)) & 0x7fu) == 0x7fu) {
-                atomicOr(&s_nan[2 + h * 4 + j / 8], 1 << (4 * (j % 8) + e));
+                atomicMin(&s_first[h * 128 + 4 * j + e], tok);
                 x[j] &= ~(0xffu << (8 * e));
               }
             }
@@ -566,7 +594,6 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         inv = den > 0.f || den != den ? 1.f / den : 0.f;
         if (p.a.lse && row_ok) p.a.lse[t * p.a.Hq + head] = den > 0.f ? top + log2f(den) : -INFINITY;
       }
-      const bool bad = s_nan[1] >= lo && s_nan[0] < hi;         // a NaN value among the row's keys
 #pragma unroll 1
       for (int d = 0; d < MT * 128; d += 32) {
         uint32_t r[32];
@@ -576,11 +603,6 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = 0u;
-        }
-        if (bad) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (s_nan[2 + d / 32] >> j & 1) r[j] = 0x7fc00000u;
         }
         if (!row_ok || d >= D) continue;
         if (part) {
@@ -600,6 +622,18 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               if (d + j < D) reinterpret_cast<uint16_t*>(o)[j] = uint16_t(w[j / 2] >> (16 * (j & 1)));
+          }
+        }
+      }
+      // a NaN value among the row's keys: its columns, over what was written. (In the loop above it cost a launch without NaN 3%.)
+      if (row_ok && s_nan[1] >= lo && s_nan[0] < hi) {
+#pragma unroll 1
+        for (int d = 0; d < D; d += 32) {
+          uint32_t nan = nan_columns(c, p.s.table + seq * p.s.ld_table, kvh, d, s_first + d, lo, min(hi, s_nan[1] + 1));
+          for (; nan; nan &= nan - 1) {
+            const int at = d + __ffs(nan) - 1;
+            if (part) part[at] = __uint_as_float(0x7fc00000u);
+            else static_cast<uint16_t*>(p.a.out)[t * p.a.o_tok + long(head) * D + at] = 0x7fc0u;
           }
         }
       }

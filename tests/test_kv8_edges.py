@@ -74,3 +74,31 @@ def test_prompt_far_apart_scales(device, sharp):
     q = randn(new, 8, 64, seed=5).mul(sharp).bfloat16()
     want, tol, _, _ = attend(q, cache, table, [n], [new], 0.125)
     near(call(device, q, cache, table, [n], [new], 0.125), want, tol)
+
+
+# ---------------------------------------------------------------------------------------------------- NaN values in prompts
+NANS = [  # page, heads, kv heads, dk, dv, length, new, window, {(position, column)}
+    (64, 8, 1, 128, 128, 600, 600, 0, [(10, 0), (481, 7), (500, 5), (505, 0)]),
+    (64, 8, 1, 128, 128, 600, 600, 100, [(385, 3), (500, 3), (500, 5), (20, 9)]),
+    (16, 16, 2, 256, 256, 400, 90, 0, [(5, 255), (330, 0), (399, 200)]),
+    (16, 16, 2, 256, 256, 400, 90, 40, [(290, 17), (350, 17), (330, 255), (371, 255)]),
+    (8, 6, 2, 64, 176, 300, 300, 33, [(t, (7 * t) % 176) for t in range(0, 300, 9)]),
+    (32, 10, 1, 80, 48, 260, 260, 7, [(t, 3) for t in range(0, 260, 20)] + [(100, c) for c in range(48)]),
+    (64, 8, 2, 64, 64, 3000, 20, 0, [(3, 1), (1500, 1), (2990, 2), (2999, 63)]),
+    (64, 8, 2, 64, 64, 3000, 20, 1100, [(1882, 1), (1890, 33), (2400, 2), (2990, 33)]),
+    (64, 4, 2, 192, 64, 200, 30, 1, [(171, 4), (180, 5), (199, 6)]),
+]
+
+
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("page,heads,kv,dk,dv,n,new,window,nans", NANS)
+def test_prompt_nan_values_reach_the_rows_that_see_them(device, page, heads, kv, dk, dv, n, new, window, nans):
+    """Several NaN values: a row is NaN in the columns of those it sees, and in no others."""
+    cache, table = filled([n], page, kv, dk, dv, seed=6, device=device)
+    for t, c in nans:
+        cache.v.view(torch.uint8)[table[0][t // page], kv - 1, t % page, c] = NAN
+    q = randn(new, heads, dk, seed=7).bfloat16()
+    want, tol, _, _ = attend(q, cache, table, [n], [new], dk ** -0.5, window=window)
+    assert bool(want.isnan().any()) and not bool(want.isnan().all())
+    near(call(device, q, cache, table, [n], [new], dk ** -0.5, window=window), want, tol)
+    assert status(device) == 0
