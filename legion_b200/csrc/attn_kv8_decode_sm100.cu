@@ -280,7 +280,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (slot == 0) {
           // a page behind the sequence, or a block outside the cache: rows that TMA fills with zeros
           row = int(next >= 0 ? next : long(c.n_blocks) * c.Hkv) * c.page;
-          sc = next_sc;
+          sc = val ? kv8_value_scale(next_sc) : next_sc;
           if (j + fill < n) {
             next = unit_of(s, j + fill);
           } else if (s.left > n) {

@@ -152,36 +152,46 @@ __device__ __forceinline__ void row_of_tile(uint32_t my_S, const float4* sc, flo
   top = fmaxf(mx0, mx1);
 }
 
-// Columns d .. d + 31 in which a key of [lo, hi) has a NaN value, a bit each. `first`: the first such key of each column. Where it
-// lies in front of the row's window, the codes of the window are looked through.
-__device__ __forceinline__ uint32_t nan_columns(const Kv8Cache& c, const int* table, int kvh, int d, const int* first, int lo, int hi) {
-  uint32_t seen = 0, look = 0;
+// Writes NaN over a row's results in the columns in which one of its keys [lo, hi) has a NaN value. `first`: the first such key of each
+// column. Where that lies in front of the row's window, the codes of the window are looked through. (Not inlined: it runs rarely, and
+// inside the loop that writes the results it cost every launch 3%.)
+__device__ __noinline__ void nan_columns(const Kv8Cache& c, const int* table, int kvh, const int* first, int lo, int hi, float* part,
+                                         uint16_t* out) {
 #pragma unroll 1
-  for (int j = 0; j < 32; ++j) {
-    const int f = first[j];
-    if (f < lo) look |= 1u << j;
-    else if (f < hi) seen |= 1u << j;
-  }
+  for (int d = 0; d < c.dv; d += 16) {
+    uint32_t seen = 0, look = 0;
 #pragma unroll 1
-  for (int tok = lo; tok < hi && look; ++tok) {
-    const int blk = table[tok / c.page];
-    if (unsigned(blk) >= unsigned(c.n_blocks)) continue;
-    const uint8_t* src = c.v + ((long(blk) * c.Hkv + kvh) * c.page + tok % c.page) * c.dv + d;
-    uint32_t found = 0;
-#pragma unroll 1
-    for (int k = 0; k < 32 && d + k < c.dv; k += 4) {
-      const uint32_t m = (*reinterpret_cast<const uint32_t*>(src + k) & 0x7f7f7f7fu) + 0x01010101u;
-      found |= ((m >> 7 & 1u) | (m >> 14 & 2u) | (m >> 21 & 4u) | (m >> 28 & 8u)) << k;
+    for (int j = 0; j < 16; ++j) {
+      const int f = first[d + j];
+      if (f < lo) look |= 1u << j;
+      else if (f < hi) seen |= 1u << j;
     }
-    seen |= found & look;
-    look &= ~found;
+#pragma unroll 1
+    for (int tok = lo; tok < hi && look; ++tok) {
+      const int blk = table[tok / c.page];
+      if (unsigned(blk) >= unsigned(c.n_blocks)) continue;
+      const uint4 u = *reinterpret_cast<const uint4*>(c.v + ((long(blk) * c.Hkv + kvh) * c.page + tok % c.page) * c.dv + d);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      uint32_t found = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t m = (w[k] & 0x7f7f7f7fu) + 0x01010101u;
+        found |= ((m >> 7 & 1u) | (m >> 14 & 2u) | (m >> 21 & 4u) | (m >> 28 & 8u)) << (4 * k);
+      }
+      seen |= found & look;
+      look &= ~found;
+    }
+    for (; seen; seen &= seen - 1) {
+      const int at = d + __ffs(seen) - 1;
+      if (part) part[at] = __uint_as_float(0x7fc00000u);
+      else out[at] = 0x7fc0u;
+    }
   }
-  return seen;
 }
 
 template <int KH, int MT, bool CAP, bool WIDE>
 __global__ void __launch_bounds__(PCfg<KH, MT>::THREADS, 1)
-kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const PromptArgs p) {
+kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PromptArgs p) {
   using C = PCfg<KH, MT>;
   constexpr int RT = C::RT, KS = C::KS, V8S = C::V8S, V16S = C::V16S, BKV = 128;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -365,7 +375,7 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         {
           const int g = at * ppb + (lane & 15) * 8 / c.page;
           const float a = __shfl_sync(0xffffffffu, ks_reg, g), b = __shfl_sync(0xffffffffu, vs_reg, g);
-          const int ev = kv8_log2(b);
+          const int ev = kv8_log2(kv8_value_scale(b));
           if (lane < 16) s_sc[(i & 3) * 16 + lane] = make_float4(a, float(ev), __uint_as_float(uint32_t(127 - ev) << 23), 0.f);
           mbar_arrive(&sc_full[i & 3]);
         }
@@ -625,18 +635,9 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           }
         }
       }
-      // a NaN value among the row's keys: its columns, over what was written. (In the loop above it cost a launch without NaN 3%.)
-      if (row_ok && s_nan[1] >= lo && s_nan[0] < hi) {
-#pragma unroll 1
-        for (int d = 0; d < D; d += 32) {
-          uint32_t nan = nan_columns(c, p.s.table + seq * p.s.ld_table, kvh, d, s_first + d, lo, min(hi, s_nan[1] + 1));
-          for (; nan; nan &= nan - 1) {
-            const int at = d + __ffs(nan) - 1;
-            if (part) part[at] = __uint_as_float(0x7fc00000u);
-            else static_cast<uint16_t*>(p.a.out)[t * p.a.o_tok + long(head) * D + at] = 0x7fc0u;
-          }
-        }
-      }
+      if (row_ok && s_nan[1] >= lo && s_nan[0] < hi)
+        nan_columns(c, p.s.table + seq * p.s.ld_table, kvh, s_first, lo, min(hi, s_nan[1] + 1), part,
+                    static_cast<uint16_t*>(p.a.out) + t * p.a.o_tok + long(head) * D);
     }
   }
   tc_fence_before();
