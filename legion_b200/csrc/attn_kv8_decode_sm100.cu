@@ -182,8 +182,8 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   griddep_launch();
   auto read_seq = [&](int b) -> int2 {
     const int row = p.s.cu[b], end = p.s.cu[b + 1];
-    const int ctx = int(min(long(max(p.s.ctx[b], 0)), long(p.s.width) * c.page));
-    const bool good = row >= 0 && end <= p.s.T && end <= row + 1;
+    const int ctx = max(p.s.ctx[b], 0);
+    const bool good = row >= 0 && end <= p.s.T && end <= row + 1 && (end <= row || ctx <= long(p.s.width) * c.page);
     if (!good && blockIdx.x == 0) atomicCAS(p.s.status, 0, ST_BAD_ARGS);
     return make_int2(ctx, good && end == row + 1 ? row : -1);
   };

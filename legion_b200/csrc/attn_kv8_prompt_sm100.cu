@@ -229,8 +229,8 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   // tiles are handed out from the last to the first: the last sees the most keys
   const int row0 = (int(gridDim.x) - 1 - int(blockIdx.x)) * (RT * 128);
   if (n_new <= 0 || row0 >= n_new * G) return;
-  const int ctx = int(min(long(max(p.s.ctx[seq], 0)), long(p.s.width) * c.page));
-  if (q0 < 0 || long(q0) + n_new > p.s.T || n_new > p.s.max_new) {
+  const int ctx = max(p.s.ctx[seq], 0);
+  if (q0 < 0 || long(q0) + n_new > p.s.T || n_new > p.s.max_new || ctx > long(p.s.width) * c.page) {
     if (threadIdx.x == 0) atomicCAS(p.s.status, 0, ST_BAD_ARGS);
     return;
   }

@@ -16,7 +16,8 @@ struct Kv8Cache {
 };
 
 // Sequences of a call: sequence i owns query (or new) rows cu[i] .. cu[i + 1], the last of its ctx[i] tokens, which lie in the
-// blocks of row i of the table.
+// blocks of row i of the table. A length beyond the table: kv8_append leaves out the rows behind it, attention the sequence, which it
+// records (ST_BAD_ARGS).
 struct Kv8Seqs {
   const int* table; long ld_table; int width;
   const int* ctx; const int* cu;

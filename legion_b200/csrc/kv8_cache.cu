@@ -53,11 +53,12 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
   const int b = blockIdx.y, h = (blockIdx.x >> 1) % c.Hkv, j = (blockIdx.x >> 1) / c.Hkv;
   const bool val = blockIdx.x & 1;
   const int row0 = p.s.cu[b], n = p.s.cu[b + 1] - row0;
-  const int ctx = int(min(long(max(p.s.ctx[b], 0)), long(p.s.width) * c.page));
-  const int first = max(ctx - n, 0);                         // position of the first new token that lies in the table
+  const int len = max(p.s.ctx[b], 0), ctx = int(min(long(len), long(p.s.width) * c.page));
+  const int first = max(len - n, 0);                         // position of the first new token
+  if (n <= 0 || first >= ctx) return;
   const int col = first / c.page + j;
   const int lo = max(first, col * c.page), hi = min(ctx, (col + 1) * c.page);
-  if (n <= 0 || lo >= hi) return;
+  if (lo >= hi) return;
   if (row0 < 0 || long(row0) + n > p.s.T || n > p.s.max_new) {
     if (threadIdx.x == 0) atomicCAS(p.s.status, 0, ST_BAD_ARGS);
     return;
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv8_append_kernel(const Append
   const int D = val ? c.dv : c.dk, per = D / 8;
   const long tok = val ? p.a.v_tok : p.a.k_tok;
   const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(val ? p.a.v : p.a.k) + (val ? p.a.v_head : p.a.k_head) * h +
-                             (row0 + (lo - (ctx - n))) * tok;
+                             (row0 + (lo - (len - n))) * tok;
   const int nvec = (hi - lo) * per;
   uint4 x[VPT];                                             // on their way while the table answers
   uint32_t m = 0;

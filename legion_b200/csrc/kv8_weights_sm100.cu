@@ -44,11 +44,12 @@ __device__ __forceinline__ Rows rows_of(const WeightArgs& p, int seq, int G) {
   Rows r;
   r.q0 = p.s.cu[seq];
   const int n_new = p.s.cu[seq + 1] - r.q0;
-  r.ctx = int(min(long(max(p.s.ctx[seq], 0)), long(p.s.width) * p.c.page));
+  r.ctx = max(p.s.ctx[seq], 0);
   r.first = p.observe > 0 ? max(0, n_new - p.observe) : 0;
   r.base = r.ctx - n_new + r.first;
   r.rows = (n_new - r.first) * G;
-  if (n_new <= 0 || r.q0 < 0 || long(r.q0) + n_new > p.s.T || n_new > p.s.max_new || r.ctx > p.w_keys) {
+  if (n_new <= 0 || r.q0 < 0 || long(r.q0) + n_new > p.s.T || n_new > p.s.max_new || r.ctx > p.w_keys ||
+      r.ctx > long(p.s.width) * p.c.page) {
     if (threadIdx.x == 0 && n_new > 0) atomicCAS(p.s.status, 0, ST_BAD_ARGS);
     r.rows = 0;
   }
@@ -325,9 +326,8 @@ __global__ void __launch_bounds__(SUM_THREADS) kv8_score_sums_kernel(const Weigh
   griddep_wait();
   griddep_launch();
   const int G = p.a.Hq / p.c.Hkv, kvh = blockIdx.y, seq = blockIdx.z;
-  const int row = p.s.cu[seq], next = p.s.cu[seq + 1], len = p.s.ctx[seq];
-  if (row < 0 || row >= p.s.T || next != row + 1) return;
-  const int ctx = int(min(long(max(len, 0)), long(p.s.width) * p.c.page));
+  const int row = p.s.cu[seq], next = p.s.cu[seq + 1], ctx = max(p.s.ctx[seq], 0);
+  if (row < 0 || row >= p.s.T || next != row + 1 || ctx > long(p.s.width) * p.c.page) return;
   const int start = (p.a.window > 0 && ctx > p.a.window) ? ctx - p.a.window : 0, base = start / BKV * BKV;
   if (ctx > p.w_keys || ctx - base > span) {
     if (threadIdx.x == 0) atomicCAS(p.s.status, 0, ST_BAD_ARGS);

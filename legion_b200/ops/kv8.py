@@ -9,8 +9,10 @@ exactly. NaN is stored as NaN; infinities count as the largest finite bf16 value
 Sequences are given as everywhere in ``ops``: ``block_table`` int32 [sequences, blocks], ``ctx_lens`` int32 the tokens a sequence
 holds with the call's rows, ``cu_q`` int32 [sequences + 1] bounds of its rows, which are the last of its tokens. On CUDA every
 call enqueues on the current stream, takes its scratch from the allocator (calls on other streams and captured graphs share none)
-and checks shapes, types and devices; what is wrong with them raises ValueError. Table entries outside the cache are not followed:
-the kernels record them in the workspace's status word. CPU tensors run the float32 forms of ``ops.reference``.
+and checks shapes, types and devices; what is wrong with them raises ValueError. What lies in tensors is checked by the kernels, which
+record it in the workspace's status word: table entries outside the cache are not followed, attention leaves out a sequence whose rows or
+length do not fit the call, its table or its sums, eviction takes a length only as far as these reach. CPU tensors run the float32 forms
+of ``ops.reference``, where such a length raises ValueError.
 """
 from __future__ import annotations
 
@@ -61,6 +63,14 @@ def _check(cache: Kv8Cache, who: str):
             raise ValueError(f"{who}: scales are float32 [blocks, kv heads]")
 
 
+def _check_lengths(cache: Kv8Cache, block_table, ctx_lens, has_rows, weights, who: str):
+    n = int(torch.where(has_rows, ctx_lens, torch.zeros_like(ctx_lens)).amax()) if ctx_lens.numel() else 0
+    if n > block_table.shape[1] * cache.page:
+        raise ValueError(f"{who}: lengths beyond the block table")
+    if weights is not None and n > weights.shape[2]:
+        raise ValueError(f"{who}: lengths beyond the sums of weights")
+
+
 def _check_weights(w, cache: Kv8Cache, block_table, who: str):
     if w.dim() != 3 or w.dtype != torch.float32 or w.shape[:2] != (block_table.shape[0], cache.k.shape[1]):
         raise ValueError(f"{who}: sums of weights are float32 [sequences, kv heads, keys]")
@@ -69,7 +79,8 @@ def _check_weights(w, cache: Kv8Cache, block_table, who: str):
 def kv8_append(cache: Kv8Cache, k, v, block_table, ctx_lens, cu_q, max_q_len: int) -> None:
     """Writes the rows' keys and values (``k`` [T, kv heads, dk], ``v`` [T, kv heads, dv], rows and heads may lie apart) to the
     cache. A block that gets its first cell begins anew: its other cells become zero. In others the scale grows where a new value
-    needs it, and the older codes are rounded to it. A block that gets tokens belongs to one sequence of the call."""
+    needs it, and the older codes are rounded to it. A block that gets tokens belongs to one sequence of the call. Rows at positions
+    that the table has no block for are left out."""
     if k.is_cuda:
         _sm.ext().kv8_append(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, block_table, ctx_lens, cu_q, max_q_len,
                              _sm.Workspace.get(k.device).status)
@@ -114,6 +125,7 @@ def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: in
             _check_weights(weights, cache, block_table, "kv8_attention")
             if observe < 0:
                 raise ValueError("kv8_attention: observed rows are not negative")
+        _check_lengths(cache, block_table, ctx_lens, cu_q[1:] > cu_q[:-1], weights, "kv8_attention")
         o = _ref.kv8_attention(q, cache, block_table, ctx_lens, cu_q, scale, window, softcap, sink, weights, observe)
         return o if out is None else out.copy_(o)
     k = cache.k
@@ -149,6 +161,7 @@ def kv8_evict(cache: Kv8Cache, block_table, ctx_lens, weights, budget: int, dst_
         if budget < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget or dst_table.shape[0] != B \
                 or dst_table.shape[1] * cache.page < budget:
             raise ValueError("kv8_evict: the budget holds the first and last tokens that stay, the blocks of the result hold the budget")
+        _check_lengths(cache, block_table, ctx_lens, torch.ones_like(ctx_lens, dtype=torch.bool), weights, "kv8_evict")
         return _ref.kv8_evict(cache, block_table, ctx_lens, weights, budget, dst_table, keep_first, keep_last)
     dev = weights.device
     lens = torch.empty(B, dtype=torch.int32, device=dev)

@@ -674,7 +674,7 @@ def kv8_append(cache, k, v, block_table, ctx_lens, cu_q):
         for i in range(len(ctx_lens)):
             q0, q1, ctx = int(cu_q[i]), int(cu_q[i + 1]), int(ctx_lens[i])
             at = ctx - (q1 - q0)
-            while at < ctx:
+            while at < min(ctx, block_table.shape[1] * page):
                 end = min(ctx, (at // page + 1) * page)
                 if end <= 0:
                     at = end

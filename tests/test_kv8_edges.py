@@ -102,3 +102,60 @@ def test_prompt_nan_values_reach_the_rows_that_see_them(device, page, heads, kv,
     assert bool(want.isnan().any()) and not bool(want.isnan().all())
     near(call(device, q, cache, table, [n], [new], dk ** -0.5, window=window), want, tol)
     assert status(device) == 0
+
+
+# ---------------------------------------------------------------------------------------------- lengths beyond the block table
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("held,new,cells", [(0, 20, 16), (15, 5, 16), (16, 3, 16), (30, 20, 32), (40, 2, 32)])
+def test_append_beyond_the_table_writes_rows_where_they_belong(device, held, new, cells):
+    """Rows whose positions lie behind the table's last block are left out; the others go to their own cells."""
+    page, D, blocks = 16, 32, cells // 16
+    table = [list(range(1, blocks + 1))]
+    caches = [ops.Kv8Cache.empty(5, page, 1, D, D, device) for _ in range(2)]
+    x = randn(held + new, 1, D, seed=1).bfloat16().to(device)
+    inside = min(held, cells)
+    for c in caches:
+        ops.kv8_append(c, x[:inside], x[:inside], i32(table, device), i32([inside], device), i32([0, inside], device), inside)
+    ops.kv8_append(caches[0], x[held:], x[held:], i32(table, device), i32([held + new], device), i32([0, new], device), new)
+    fit = max(0, min(held + new, cells) - held)
+    if fit:
+        ops.kv8_append(caches[1], x[held:held + fit], x[held:held + fit], i32(table, device), i32([held + fit], device), i32([0, fit], device), fit)
+    for name in caches[0].__slots__:
+        assert torch.equal(*(getattr(c, name).view(torch.uint8) for c in caches))
+    assert status(device) == 0
+
+
+@gpu
+@pytest.mark.parametrize("window", [0, 9])
+@pytest.mark.parametrize("new", [[1, 1, 1], [10, 3, 30]])
+def test_attention_beyond_the_table_is_recorded(window, new):
+    """A sequence with more tokens than its table has blocks for is left out; the others of the call are not touched by it. (On the
+    CPU the call is refused.)"""
+    device, heads, D, lens = "cuda:0", 4, 64, [30, 65, 50]
+    cache, table = filled(lens, 16, 2, D, D, seed=8, device=device)
+    q = randn(sum(new), heads, D, seed=9).bfloat16()
+    want, tol, weight, off = attend(q, cache, table, lens, new, 0.125, window=window)
+    w, out = torch.full((3, 2, 70), 0.5, device=device), torch.full((sum(new), heads, D), 7.0, dtype=torch.bfloat16, device=device)
+    short = i32([row[:4] for row in table], device)          # 64 cells
+    ops.kv8_attention(q.to(device), cache, short, i32(lens, device), i32(cum(new), device), max(new), 0.125, window=window, weights=w, out=out)
+    assert status(device) != 0
+    mine = torch.ones(sum(new), dtype=torch.bool)
+    mine[new[0]:new[0] + new[1]] = False
+    near(out[mine.to(device)], want[mine], tol[mine])
+    assert bool((out[~mine.to(device)] == 7.0).all()) and bool((w[1] == 0.5).all())
+    for i in (0, 2):
+        got = w[i, :, :lens[i]].cpu().double() - 0.5
+        assert bool(((got - weight[i].sum(2)).abs() <= off[i].sum(2) + 2.0 ** -23 * (0.5 + weight[i].sum(2))).all())
+
+
+def test_attention_and_eviction_beyond_the_table_are_refused_on_the_cpu():
+    cache, table = filled([35], 16, 2, 32, 32)
+    short, q, w = i32([table[0][:2]]), randn(1, 4, 32).bfloat16(), torch.zeros(1, 2, 40)
+    with pytest.raises(ValueError, match="table"):
+        ops.kv8_attention(q, cache, short, i32([35]), i32([0, 1]), 1, 0.2)
+    with pytest.raises(ValueError, match="table"):
+        ops.kv8_evict(cache, short, i32([35]), w, 16, i32([[0]]))
+    with pytest.raises(ValueError, match="sums"):
+        ops.kv8_evict(cache, i32(table), i32([35]), w[..., :30], 16, i32([[0]]))
+    with pytest.raises(ValueError, match="sums"):
+        ops.kv8_attention(q, cache, i32(table), i32([35]), i32([0, 1]), 1, 0.2, weights=w[..., :30])
