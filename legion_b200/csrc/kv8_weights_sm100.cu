@@ -12,7 +12,8 @@
 // S^T[128 keys, 64 rows] = K . Q^T on tcgen05, with the terms, scales and order of the attention, whose sums its scores have to be
 // bit for bit: the tensor cores cut off what does not fit a sum, and scores summed in another order gave weights 10^-6 too large.
 // A thread has a key and adds up its columns over all records, so nothing crosses threads and the result does not depend on any
-// order but the rows' own. Two score tiles are made ahead of their use. 64 exponentials per key and record
+// order but the rows' own; what the additions of records round off is carried along (single additions of 0.88 from 20800 rows ended 2^-12
+// off: beyond 8192 all of them round the same way). Two score tiles are made ahead of their use. 64 exponentials per key and record
 // and the records' traffic bound it: 64 rows of 32 heads over 16K keys add 30 us to the call, all 1024 rows 295 (a mask branch per
 // score instead of per record and one score tile: 57 and 510).
 #include <type_traits>
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
     const int w = warp >> 2, tl = (warp & 3) * 32 + lane;
     const uint32_t my_lane = uint32_t((warp & 3) * 32) << 16;
     const int tok = key0 + w * BKV + tl;
-    float ks = 0.f, acc0 = 0.f, acc1 = 0.f;
+    float ks = 0.f, sum = 0.f, lost = 0.f;        // the key's sum and what its additions rounded off
     if (w < n_tiles && tok < x.ctx) {
       const int blk = bt[tok / c.page];
       if (unsigned(blk) < unsigned(c.n_blocks)) ks = c.k_scale[long(blk) * c.Hkv + kvh];
@@ -278,6 +279,7 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
         const int rt = ra + i, pos_a = x.base + rt * RN / G, pos_b = x.base + (min(x.rows, (rt + 1) * RN) - 1) / G;
         const int last = key0 + w * BKV + BKV - 1;
         const bool full = last < x.ctx && last <= pos_a && (p.a.window == 0 || last - BKV + 1 > pos_b - p.a.window);
+        float acc0 = 0.f, acc1 = 0.f;
         auto add_up = [&](auto masked) {
 #pragma unroll 2
           for (int r0 = 0; r0 < RN; r0 += 16) {
@@ -308,10 +310,13 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
         else add_up(std::true_type{});
         tc_fence_before();
         mbar_arrive(&s_empty[w * 2 + (i & 1)]);
+        const float more = (acc0 + acc1) - lost, now = sum + more;
+        lost = (now - sum) - more;
+        sum = now;
       }
       if (lane == 0) mbar_arrive(&r_empty[st]);
     }
-    if (ok && w < n_tiles && tok < x.ctx) p.w[seq * p.w_seq + kvh * p.w_head + tok] += acc0 + acc1;
+    if (ok && w < n_tiles && tok < x.ctx) p.w[seq * p.w_seq + kvh * p.w_head + tok] += sum;
   }
   tc_fence_before();
   __syncthreads();

@@ -159,3 +159,25 @@ def test_attention_and_eviction_beyond_the_table_are_refused_on_the_cpu():
         ops.kv8_evict(cache, i32(table), i32([35]), w[..., :30], 16, i32([[0]]))
     with pytest.raises(ValueError, match="sums"):
         ops.kv8_attention(q, cache, i32(table), i32([35]), i32([0, 1]), 1, 0.2, weights=w[..., :30])
+
+
+# --------------------------------------------------------------------------------------------------------------- long sums
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("n,heads", [(2600, 8), (1900, 16)])
+def test_sums_of_many_equal_weights(device, n, heads):
+    """A key that gets the same 0.88 from each of 20800 to 30400 rows and heads: additions that all round one way must not add up.
+    Products of the scores are exact here; a weight is off by its exponent's rounding (scores of 12 and log-sum-exps in 32 bits,
+    a step of 2^-20 each) and by the exponential's, together below 2^-18; 2^-17 is asked for."""
+    D = 16
+    k = torch.full((n, 1, D), -8.0)
+    k[0], k[1] = 1.0, 0.75
+    cache, table = holding(k, torch.ones(n, 1, D), 64, device)
+    q = torch.ones(n, heads, D, dtype=torch.bfloat16)
+    w = torch.zeros(1, 1, n, device=device)
+    call(device, q, cache, table, [n], [n], 0.5, weights=w)
+    # position 0 sees key 0 alone
+    big = heads * (1 + (n - 1) / (1 + math.exp(-2)))
+    small = heads * (n - 1) / (1 + math.exp(2))
+    got = w[0, 0].cpu().double()
+    assert abs(float(got[0]) / big - 1) <= 2.0 ** -17 and abs(float(got[1]) / small - 1) <= 2.0 ** -17
+    assert status(device) == 0
