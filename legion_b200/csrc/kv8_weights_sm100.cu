@@ -32,6 +32,8 @@ struct WeightArgs {
   Kv8Seqs s;
   Kv8Attn a;
   int observe, max_rt;            // last rows of a sequence that count (0: all); records of a sequence and head at most
+  long per_head;                  // records that a kv head has room for
+  int packed;                     // they lie in the order of the call's rows; else max_rt to a sequence
   float scale_log2, cap_k;
   float* w; long w_seq, w_head; int w_keys;
   uint8_t* records;
@@ -57,15 +59,34 @@ __device__ __forceinline__ Rows rows_of(const WeightArgs& p, int seq, int G) {
   return r;
 }
 
+// Index of a sequence's first record among its kv head's. In the order of the rows: a sequence of n rows has ceil(n G / 64) records at
+// most, and floor(q0 G / 64) + sequence leaves it that many, up to ceil(T G / 64) + sequences in all.
+__device__ __forceinline__ long first_record(const WeightArgs& p, int seq, int q0, int G) {
+  return p.packed ? long(q0) * G / RN + seq : long(seq) * p.max_rt;
+}
+
 template <int KH>
 __global__ void __launch_bounds__(256) kv8_queries_kernel(const WeightArgs p) {
   griddep_wait();
   griddep_launch();
-  const int G = p.a.Hq / p.c.Hkv, rt = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
+  const int G = p.a.Hq / p.c.Hkv, kvh = blockIdx.y;
+  int seq = blockIdx.z, rt = blockIdx.x;
+  if (p.packed) {
+    // the last sequence whose records begin here or before
+    int lo = 0, hi = p.s.n;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (first_record(p, mid, p.s.cu[mid], G) <= long(blockIdx.x)) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo == 0) return;
+    seq = lo - 1;
+    rt = int(blockIdx.x - first_record(p, seq, p.s.cu[seq], G));
+  }
   const Rows x = rows_of(p, seq, G);
+  if (long(rt) * RN >= x.rows) return;
   const int n = min(RN, x.rows - rt * RN);
-  if (n <= 0) return;
-  uint8_t* rec = p.records + ((long(seq) * p.c.Hkv + kvh) * p.max_rt + rt) * (HEAD + 2 * KH * RN * 128);
+  uint8_t* rec = p.records + (kvh * p.per_head + first_record(p, seq, x.q0, G) + rt) * (HEAD + 2 * KH * RN * 128);
   float* head = reinterpret_cast<float*>(rec);
   constexpr int PER = RN * KH * 8 / 256;                  // chunks of 16 values of a thread
 #pragma unroll 1
@@ -210,7 +231,7 @@ __global__ void __launch_bounds__(320, KH == 1 ? 2 : 1) kv8_weights_kernel(const
             tma_load_2d(k_s + t * C::K_BYTES + h * 16384 + g * c.page * 128, &tmK, &k_full[t], h * 128, (b * c.Hkv + kvh) * c.page);
       }
     }
-    const uint8_t* rec = p.records + (long(seq) * c.Hkv + kvh) * p.max_rt * C::R_BYTES;
+    const uint8_t* rec = p.records + (kvh * p.per_head + first_record(p, seq, x.q0, G)) * C::R_BYTES;
     for (int i = 0; i < rb - ra; ++i) {
       const int st = i % ST;
       if (i >= ST && !__all_sync(0xffffffffu, mbar_wait(&r_empty[st], ((i / ST) - 1) & 1, abort_flag))) {
@@ -366,7 +387,7 @@ __global__ void __launch_bounds__(SUM_THREADS) kv8_score_sums_kernel(const Weigh
 }
 
 WeightArgs make(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, float* w, long w_seq, long w_head, int w_keys) {
-  WeightArgs p{c, s, a, 0, 0, a.scale * 1.4426950408889634f, 0.f, w, w_seq, w_head, w_keys, nullptr};
+  WeightArgs p{c, s, a, 0, 0, 0, 0, a.scale * 1.4426950408889634f, 0.f, w, w_seq, w_head, w_keys, nullptr};
   if (a.softcap > 0.f) {
     p.cap_k = 2.f * 1.4426950408889634f * a.scale / a.softcap;
     p.scale_log2 = 2.f * 1.4426950408889634f * a.softcap;
@@ -379,20 +400,29 @@ cudaError_t launch(const CUtensorMap* tk, const WeightArgs& p, int tiles, cudaSt
   auto kfn = kv8_weights_kernel<KH, CAP>;
   static DeviceOnce once;
   cudaError_t e = once.shared_memory(reinterpret_cast<const void*>(kfn), WCfg<KH>::SMEM);
-  if (e == cudaSuccess) e = launch_pdl(kv8_queries_kernel<KH>, dim3(p.max_rt, p.c.Hkv, p.s.n), dim3(256), 0, st, p);
+  const dim3 records = p.packed ? dim3(unsigned(p.per_head), p.c.Hkv) : dim3(p.max_rt, p.c.Hkv, p.s.n);
+  if (e == cudaSuccess) e = launch_pdl(kv8_queries_kernel<KH>, records, dim3(256), 0, st, p);
   if (e == cudaSuccess) e = launch_pdl(kfn, dim3((tiles + 1) / 2, p.c.Hkv, p.s.n), dim3(320), WCfg<KH>::SMEM, st, *tk, p);
   return e;
 }
 
-int max_records(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int observe) {
-  const long rows = long(observe > 0 && observe < s.max_new ? observe : s.max_new) * (a.Hq / c.Hkv);
-  return int((rows + RN - 1) / RN);
+// Where the records of a call lie: by sequence, or where that has more room than its rows need (one long prompt beside 63 single tokens:
+// 4.5 GB instead of 76 MB) in their order.
+void place(WeightArgs& p, int observe) {
+  const long G = p.a.Hq / p.c.Hkv, rows = long(observe > 0 && observe < p.s.max_new ? observe : p.s.max_new) * G;
+  p.observe = observe;
+  p.max_rt = int((rows + RN - 1) / RN);
+  const long apart = long(p.s.n) * p.max_rt, packed = (p.s.T * G + RN - 1) / RN + p.s.n;
+  p.packed = packed < apart;
+  p.per_head = p.packed ? packed : apart;
 }
 
 }  // namespace
 
 int64_t kv8_weights_scratch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int observe) {
-  return int64_t(s.n) * c.Hkv * max_records(c, s, a, observe) * (HEAD + (c.dk + 127) / 128 * 2 * RN * 128);
+  WeightArgs p{c, s, a};
+  place(p, observe);
+  return int64_t(c.Hkv) * p.per_head * (HEAD + (c.dk + 127) / 128 * 2 * RN * 128);
 }
 
 int kv8_weights_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int observe, int tiles, void* scratch, float* w, long w_seq,
@@ -404,8 +434,7 @@ int kv8_weights_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, in
     return 1;
   }
   WeightArgs p = make(c, s, a, w, w_seq, w_head, w_keys);
-  p.observe = observe;
-  p.max_rt = max_records(c, s, a, observe);
+  place(p, observe);
   p.records = static_cast<uint8_t*>(scratch);
   const bool cap = a.softcap > 0.f;
   const cudaError_t e = c.dk <= 128 ? (cap ? launch<1, true>(tk, p, tiles, st) : launch<1, false>(tk, p, tiles, st))

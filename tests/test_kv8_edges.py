@@ -181,3 +181,54 @@ def test_sums_of_many_equal_weights(device, n, heads):
     got = w[0, 0].cpu().double()
     assert abs(float(got[0]) / big - 1) <= 2.0 ** -17 and abs(float(got[1]) / small - 1) <= 2.0 ** -17
     assert status(device) == 0
+
+
+# ------------------------------------------------------------------------------------------------- sums of ragged batches
+RAGGED = [  # page, heads, kv heads, D, lengths, new tokens, observed rows
+    (16, 8, 2, 64, [500] + [1] * 20, [500] + [1] * 20, 0),
+    (64, 40, 8, 64, [30, 400, 3, 0, 77], [30, 130, 3, 0, 5], 0),
+    (64, 40, 8, 64, [30, 400, 3, 0, 77], [30, 130, 3, 0, 5], 100),
+    (32, 6, 2, 96, [1, 300, 1], [1, 300, 1], 7),
+    (16, 5, 1, 160, [9] * 30 + [333], [9] * 30 + [260], 0),
+]
+
+
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("page,heads,kv,D,lens,new,observe", RAGGED)
+def test_sums_of_ragged_batches(device, page, heads, kv, D, lens, new, observe):
+    cache, table = filled(lens, page, kv, D, D, seed=31, device=device)
+    q = randn(sum(new), heads, D, seed=32).bfloat16()
+    want_o, tol_o, weight, off = attend(q, cache, table, lens, new, D ** -0.5, window=200)
+    start = torch.rand(len(lens), kv, max(lens), generator=gen(1))
+    w = start.clone().to(device)
+    near(call(device, q, cache, table, lens, new, D ** -0.5, window=200, weights=w, observe=observe), want_o, tol_o)
+    assert status(device) == 0
+    for i, (n, m) in enumerate(zip(lens, new)):
+        rows = torch.arange(weight[i].shape[2]) % max(m, 1) >= (m - observe if observe else 0)
+        want, tol = weight[i][:, :, rows].sum(2), off[i][:, :, rows].sum(2)
+        got = w[i].cpu().double() - start[i].double()
+        assert bool(((got[:, :n] - want).abs() <= tol + 2.0 ** -23 * (start[i, :, :n] + want)).all())
+        assert not bool(got[:, n:].any())
+
+
+@gpu
+@pytest.mark.parametrize("observe", [0, 64])
+def test_sums_of_a_ragged_batch_take_scratch_by_its_rows(observe):
+    """One long prompt beside 63 single tokens: 8255 rows of 8 heads a kv head, 17 KB for every 64 of them, not 64 times the longest."""
+    device, lens = "cuda:0", [8192] + [1] * 63
+    cache, table = filled(lens, 64, 4, 64, 64, seed=3, device=device)
+    q = randn(sum(lens), 32, 64, seed=4).bfloat16().to(device)
+    w = torch.zeros(64, 4, 8192, device=device)
+    args = (q, cache, i32(table, device), i32(lens, device), i32(cum(lens), device), 8192, 0.125)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.kv8_attention(*args, weights=w, observe=observe)
+    # records of both codings of the rows (256 bytes a row and head of 128 columns, 16 for its scale, log-sum-exp and position), the
+    # output, log-sum-exps, and one record of 64 rows more for every sequence and head
+    rows = (sum(lens) if observe == 0 else min(sum(lens), 64 * observe)) * 32
+    assert torch.cuda.max_memory_allocated() - before <= 2 * (rows * 272 + 64 * 4 * 64 * 272) + q.numel() * 2 + sum(lens) * 32 * 4 + (1 << 22)
+    # softmax weights: every row and head gives 1
+    total = float(w.double().sum())
+    rows = [min(n, observe) if observe else n for n in lens]
+    assert abs(total - 32 * sum(rows)) <= 2.0 ** -16 * 32 * sum(rows) and status(device) == 0
