@@ -56,11 +56,29 @@ class Kv8Cache:
 
 def _check(cache: Kv8Cache, who: str):
     k, v = cache.k, cache.v
+    if k.is_cuda:
+        raise ValueError(f"{who}: tensors on different devices")
     if k.dim() != 4 or v.dim() != 4 or k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn or k.shape[:3] != v.shape[:3]:
         raise ValueError(f"{who}: codes are float8_e4m3fn [blocks, kv heads, page, head size]")
     for s in (cache.k_scale, cache.v_scale):
         if s.dtype != torch.float32 or s.shape != k.shape[:2]:
             raise ValueError(f"{who}: scales are float32 [blocks, kv heads]")
+
+
+def _sizes(cache: Kv8Cache, rows, block_table, who: str):
+    """(sequences, table width, kv heads, page, dk, dv) and the sizes of ``rows``: what the front ends rely on. The extension checks
+    the rest."""
+    try:
+        n, width = block_table.shape
+        _, kv, page, dk = cache.k.shape
+        _, _, _, dv = cache.v.shape
+        _, heads, cols = rows.shape
+    except ValueError:
+        raise ValueError(f"{who}: codes are [blocks, kv heads, page, head size], block tables [sequences, blocks], rows or sums have three "
+                         "dimensions") from None
+    if kv < 1 or page < 1 or heads < 1:
+        raise ValueError(f"{who}: a cache and rows without heads or cells")
+    return n, width, kv, page, dk, dv, heads, cols
 
 
 def _check_lengths(cache: Kv8Cache, block_table, ctx_lens, has_rows, weights, who: str):
@@ -81,9 +99,9 @@ def kv8_append(cache: Kv8Cache, k, v, block_table, ctx_lens, cu_q, max_q_len: in
     cache. A block that gets its first cell begins anew: its other cells become zero. In others the scale grows where a new value
     needs it, and the older codes are rounded to it. A block that gets tokens belongs to one sequence of the call. Rows at positions
     that the table has no block for are left out."""
-    if k.is_cuda:
+    if k.is_cuda or cache.k.is_cuda:
         _sm.ext().kv8_append(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, block_table, ctx_lens, cu_q, max_q_len,
-                             _sm.Workspace.get(k.device).status)
+                             _sm.Workspace.get(cache.k.device).status)
         return
     _check(cache, "kv8_append")
     if k.dim() != 3 or v.dim() != 3 or k.shape[:2] != v.shape[:2] or k.shape[1:] != cache.k.shape[1::2] or v.shape[1:] != cache.v.shape[1::2]:
@@ -115,9 +133,10 @@ def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: in
     share its head and over the sequence's last ``observe`` rows (0: all of the call), is added to its sum: what ``kv8_evict`` goes
     by. The sums do not depend on the order of anything but the rows. A decode call with sums takes 4 bytes of scratch per row, head
     and key up to ``max_ctx``."""
+    n, width, kv, page, dk, dv, heads, cols = _sizes(cache, q, block_table, "kv8_attention")
     if not q.is_cuda:
         _check(cache, "kv8_attention")
-        if q.dim() != 3 or q.shape[2] != cache.k.shape[3] or q.shape[1] % cache.k.shape[1]:
+        if cols != dk or heads % kv:
             raise ValueError("kv8_attention: queries [T, heads, head size] do not fit the cache")
         if window < 0 or softcap < 0:
             raise ValueError("kv8_attention: window and soft cap are not negative")
@@ -128,20 +147,18 @@ def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: in
         _check_lengths(cache, block_table, ctx_lens, cu_q[1:] > cu_q[:-1], weights, "kv8_attention")
         o = _ref.kv8_attention(q, cache, block_table, ctx_lens, cu_q, scale, window, softcap, sink, weights, observe)
         return o if out is None else out.copy_(o)
-    k = cache.k
     if out is None:
-        out = torch.empty(q.shape[0], q.shape[1], cache.v.shape[3], dtype=q.dtype, device=q.device)
-    span = min(max_ctx or 1 << 30, block_table.shape[1] * k.shape[2])
-    tiles = max(1, -(-span // 128))
+        out = torch.empty(q.shape[0], heads, dv, dtype=q.dtype, device=q.device)
+    tiles = max(1, -(-min(max_ctx or 1 << 30, width * page) // 128))
     if window > 0 and max_q_len == 1:
         tiles = min(tiles, -(-window // 128) + 1)
-    group = q.shape[1] // k.shape[1]
+    group = heads // kv
     if max_q_len == 1:
-        splits = min(_sm.NUM_SMS, block_table.shape[0] * k.shape[1] * -(-group // (8 if group <= 8 else 16)) * tiles)      # CTAs
+        splits = min(_sm.NUM_SMS, n * kv * -(-group // (8 if group <= 8 else 16)) * tiles)      # CTAs
     else:
-        rows = 256 if k.shape[3] <= 128 and cache.v.shape[3] <= 128 else 128
-        splits = _prompt_splits(block_table.shape[0], k.shape[1], max_q_len * group, rows, tiles if window <= 0 else min(tiles, (window + max_q_len) // 128 + 1))
-    _sm.ext().kv8_attention(q, k, cache.v, cache.k_scale, cache.v_scale, block_table, ctx_lens, cu_q, max_q_len, scale, window,
+        rows = 256 if dk <= 128 and dv <= 128 else 128
+        splits = _prompt_splits(n, kv, max_q_len * group, rows, tiles if window <= 0 else min(tiles, (window + max_q_len) // 128 + 1))
+    _sm.ext().kv8_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, ctx_lens, cu_q, max_q_len, scale, window,
                             softcap, sink, splits, out, _sm.Workspace.get(q.device).status, weights, observe, tiles)
     return out
 
@@ -154,19 +171,19 @@ def kv8_evict(cache: Kv8Cache, block_table, ctx_lens, weights, budget: int, dst_
 
     Returns (lengths int32 [sequences], the kept tokens' places before int32 [sequences, kv heads, budget], -1 behind the last, and
     their sums float32 likewise, 0 behind the last)."""
-    B, kv = block_table.shape[0], cache.k.shape[1]
+    B, _, kv, page, _, _, _, _ = _sizes(cache, weights, block_table, "kv8_evict")
+    if budget < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget or dst_table.dim() != 2 \
+            or dst_table.shape[0] != B or dst_table.shape[1] * page < budget:
+        raise ValueError("kv8_evict: the budget holds the first and last tokens that stay, the blocks of the result hold the budget")
     if not weights.is_cuda:
         _check(cache, "kv8_evict")
         _check_weights(weights, cache, block_table, "kv8_evict")
-        if budget < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget or dst_table.shape[0] != B \
-                or dst_table.shape[1] * cache.page < budget:
-            raise ValueError("kv8_evict: the budget holds the first and last tokens that stay, the blocks of the result hold the budget")
         _check_lengths(cache, block_table, ctx_lens, torch.ones_like(ctx_lens, dtype=torch.bool), weights, "kv8_evict")
         return _ref.kv8_evict(cache, block_table, ctx_lens, weights, budget, dst_table, keep_first, keep_last)
     dev = weights.device
     lens = torch.empty(B, dtype=torch.int32, device=dev)
-    kept = torch.empty(B, kv, max(0, budget), dtype=torch.int32, device=dev)
-    sums = torch.empty(B, kv, max(0, budget), device=dev)
+    kept = torch.empty(B, kv, budget, dtype=torch.int32, device=dev)
+    sums = torch.empty(B, kv, budget, device=dev)
     _sm.ext().kv8_evict(cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, ctx_lens, weights, budget, keep_first, keep_last,
                         dst_table, lens, kept, sums, _sm.Workspace.get(dev).status)
     return lens, kept, sums

@@ -232,3 +232,50 @@ def test_sums_of_a_ragged_batch_take_scratch_by_its_rows(observe):
     total = float(w.double().sum())
     rows = [min(n, observe) if observe else n for n in lens]
     assert abs(total - 32 * sum(rows)) <= 2.0 ** -16 * 32 * sum(rows) and status(device) == 0
+
+
+# --------------------------------------------------------------------------------------------------------- malformed calls
+BAD = {  # what: change of the call's arguments
+    "queries of two dimensions": lambda a: a.update(q=a["q"][0]),
+    "keys of three dimensions": lambda a: setattr(a["cache"], "k", a["cache"].k[0]),
+    "values of three dimensions": lambda a: setattr(a["cache"], "v", a["cache"].v[0]),
+    "a cache without heads": lambda a: [setattr(a["cache"], n, getattr(a["cache"], n)[:, :0]) for n in a["cache"].__slots__],
+    "a table of one dimension": lambda a: a.update(table=a["table"][0]),
+    "no query heads": lambda a: a.update(q=a["q"][:, :0]),
+    "head size": lambda a: a.update(q=a["q"][..., :16]),
+}
+
+
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("what", list(BAD))
+def test_malformed_calls_are_value_errors(device, new, what):
+    cache, table = filled([20], 16, 2, 32, 32, device=device)
+    a = dict(cache=cache, q=randn(new, 4, 32).bfloat16().to(device), table=i32(table, device))
+    BAD[what](a)
+    with pytest.raises(ValueError, match="kv8_attention"):
+        ops.kv8_attention(a["q"], a["cache"], a["table"], i32([20], device), i32([0, new], device), new, 0.2)
+    if "quer" not in what and what != "head size":
+        with pytest.raises(ValueError, match="kv8_evict"):
+            ops.kv8_evict(a["cache"], a["table"], i32([20], device), torch.zeros(1, 2, 20, device=device), 16, i32([[1]], device))
+
+
+@gpu
+def test_a_cache_and_rows_on_different_devices():
+    device = "cuda:0"
+    cache, table = filled([20], 16, 2, 32, 32, device=device)
+    q, k, where = randn(1, 4, 32).bfloat16(), randn(1, 2, 32).bfloat16(), (i32(table), i32([20]), i32([0, 1]))
+    with pytest.raises(ValueError, match="devices"):
+        ops.kv8_attention(q, cache, *where, 1, 0.2)
+    with pytest.raises(ValueError, match="devices"):
+        ops.kv8_append(cache, k, k, *where, 1)
+    with pytest.raises(ValueError, match="devices"):
+        ops.kv8_evict(cache, *where[:2], torch.zeros(1, 2, 20), 16, i32([[1]]))
+
+
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("budget", [0, -1, 17, 1 << 45])
+def test_budgets_are_checked_before_results_are_allocated(device, budget):
+    cache, table = filled([20], 16, 2, 32, 32, device=device)
+    with pytest.raises(ValueError, match="kv8_evict"):
+        ops.kv8_evict(cache, i32(table, device), i32([20], device), torch.zeros(1, 2, 20, device=device), budget, i32([[1]], device))
