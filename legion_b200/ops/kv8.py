@@ -160,6 +160,8 @@ def kv8_attention(q, cache: Kv8Cache, block_table, ctx_lens, cu_q, max_q_len: in
         splits = _prompt_splits(n, kv, max_q_len * group, rows, tiles if window <= 0 else min(tiles, (window + max_q_len) // 128 + 1))
     _sm.ext().kv8_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, ctx_lens, cu_q, max_q_len, scale, window,
                             softcap, sink, splits, out, _sm.Workspace.get(q.device).status, weights, observe, tiles)
+    # kernels beside the attention's own: the join of the parts, the sums (of prompt rows: their records first)
+    _sm.LAUNCHES["n"] += (splits > 1) + (0 if weights is None else 1 if max_q_len == 1 else 2)
     return out
 
 

@@ -279,3 +279,25 @@ def test_budgets_are_checked_before_results_are_allocated(device, budget):
     cache, table = filled([20], 16, 2, 32, 32, device=device)
     with pytest.raises(ValueError, match="kv8_evict"):
         ops.kv8_evict(cache, i32(table, device), i32([20], device), torch.zeros(1, 2, 20, device=device), budget, i32([[1]], device))
+
+
+# ---------------------------------------------------------------------------------------------------------------- launches
+@gpu
+@pytest.mark.parametrize("lens,new,sums", [([1000], [1], False), ([1000], [1], True), ([10], [1], True), ([3000], [5], False), ([3000], [5], True),
+                                           ([200] * 60, [200] * 60, True)])
+def test_launches_are_counted(lens, new, sums):
+    """The launch counter against the kernels of the captured call."""
+    runtime = pytest.importorskip("cuda.bindings.runtime")
+    device = "cuda:0"
+    cache, table = filled(lens, 64, 1, 64, 64, device=device)
+    q = randn(sum(new), 4, 64).bfloat16().to(device)
+    args = (q, cache, i32(table, device), i32(lens, device), i32(cum(new), device), max(new), 0.125)
+    w = torch.zeros(len(lens), 1, max(lens), device=device) if sums else None
+    before = ops.sm100.LAUNCHES["n"]
+    ops.kv8_attention(*args, weights=w)
+    counted = ops.sm100.LAUNCHES["n"] - before
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g):
+        ops.kv8_attention(*args, weights=w)
+    err, _, n = runtime.cudaGraphGetNodes(g.raw_cuda_graph())
+    assert int(err) == 0 and n == counted
