@@ -93,6 +93,7 @@ void kv8_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
          ": window and soft cap are not negative, the scale is finite");
   LB_ASK(out.scalar_type() == at::kBFloat16 && out.dim() == 3 && out.size(0) == T && out.size(1) == Hq && out.size(2) == c.dv &&
              out.stride(2) == 1 && (out.stride(1) == c.dv || Hq == 1), who, ": out is bfloat16 [rows, heads, value head size]");
+  LB_ASK(T <= 1 || out.stride(0) >= Hq * c.dv, who, ": rows of out overlap");
   lb::Kv8Attn a{q.data_ptr(), long(q.stride(0)), long(q.stride(1)), int(Hq), float(scale), float(softcap), int(window), nullptr,
                 out.data_ptr(), long(out.stride(0)), nullptr, nullptr, 0};
   if (sink.has_value()) {

@@ -301,3 +301,16 @@ def test_launches_are_counted(lens, new, sums):
         ops.kv8_attention(*args, weights=w)
     err, _, n = runtime.cudaGraphGetNodes(g.raw_cuda_graph())
     assert int(err) == 0 and n == counted
+
+
+# ------------------------------------------------------------------------------------------------------------------- outputs
+def test_output_rows_that_overlap_are_refused():
+    if not ops.sm100.have_ext():
+        pytest.skip("extension not built")
+    cache, table = filled([20], 16, 2, 32, 32)
+    C, st = ops.sm100.ext(), torch.zeros(4, dtype=torch.int32)
+    q = randn(3, 4, 32).bfloat16()
+    for out in (torch.zeros(1, 4, 32, dtype=torch.bfloat16).expand(3, 4, 32), torch.zeros(300, dtype=torch.bfloat16).as_strided((3, 4, 32), (64, 32, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            C.kv8_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, i32(table), i32([20]), i32([0, 3]), 3, 0.1, 0, 0.0, None, 1,
+                            out, st, None, 0, 1)
