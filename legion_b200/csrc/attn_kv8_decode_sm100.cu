@@ -752,12 +752,19 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const DecodeArgs p, in
        [&](int i) { return p.part + ((long(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * nq + q) * stride; }, s_w);
 }
 
-// Prompt rows: every part of every row and head is there
-__global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8Seqs s, const Kv8Attn a, int D, int n_splits, const float* part) {
+// Prompt rows: every part of every row and head is there, but for rows of no sequence and of those that the attention leaves out
+__global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8Seqs s, const Kv8Attn a, int page, int D, int n_splits, const float* part) {
   __shared__ float s_w[256];
   const int h = blockIdx.x % a.Hq;
   const long row = blockIdx.x / a.Hq;
-  if (row < s.cu[0] || row >= s.cu[s.n]) return;           // a row of no sequence
+  int seq = 0;                                             // the last sequence that begins here or before
+  for (int end = s.n; end - seq > 1;) {
+    const int mid = (seq + end) / 2;
+    if (s.cu[mid] <= row) seq = mid;
+    else end = mid;
+  }
+  const int q0 = s.cu[seq], q1 = s.cu[seq + 1];
+  if (q0 < 0 || row < q0 || row >= q1 || q1 > s.T || q1 - q0 > s.max_new || s.ctx[seq] > long(s.width) * page) return;
   join(a, D, row, h, n_splits, [&](int i) { return part + ((row * a.Hq + h) * n_splits + i) * (D + 2); }, s_w);
 }
 
@@ -774,7 +781,7 @@ cudaError_t launch(const CUtensorMap* tk, const CUtensorMap* tv, const DecodeArg
 }  // namespace
 
 cudaError_t kv8_join(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int n_splits, float* part, cudaStream_t st) {
-  kv8_join_kernel<<<unsigned(s.T * a.Hq), 128, 0, st>>>(s, a, c.dv, n_splits, part);
+  kv8_join_kernel<<<unsigned(s.T * a.Hq), 128, 0, st>>>(s, a, c.page, c.dv, n_splits, part);
   return cudaGetLastError();
 }
 

@@ -314,3 +314,57 @@ def test_output_rows_that_overlap_are_refused():
         with pytest.raises(ValueError, match="overlap"):
             C.kv8_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, i32(table), i32([20]), i32([0, 3]), 3, 0.1, 0, 0.0, None, 1,
                             out, st, None, 0, 1)
+
+
+@gpu
+@pytest.mark.parametrize("fault", ["length", "rows"])
+def test_rows_that_are_left_out_stay_as_they_were(fault):
+    """Where the keys of a prompt call are split, the join leaves the rows of a sequence that was left out alone, too."""
+    device, heads, D, lens, new = "cuda:0", 4, 64, [1500, 1700, 0, 1200], [5, 9, 0, 2]
+    cache, table = filled(lens, 16, 2, D, D, seed=8, device=device)
+    q = randn(sum(new), heads, D, seed=9).bfloat16()
+    want, tol, _, _ = attend(q, cache, table, lens, new, 0.125)
+    most = 9 if fault == "length" else 8                     # (a sequence with more rows than the call allows)
+    width = 100 if fault == "length" else len(table[0])      # (1600 cells)
+    assert ops.kv8._prompt_splits(4, 2, most * 2, 256, 13) > 1
+    out = torch.full((sum(new), heads, D), 7.0, dtype=torch.bfloat16, device=device)
+    ops.kv8_attention(q.to(device), cache, i32([row[:width] for row in table], device), i32(lens, device), i32(cum(new), device), most, 0.125,
+                      max_ctx=1700, out=out)
+    assert status(device) != 0
+    mine = torch.ones(sum(new), dtype=torch.bool)
+    mine[5:14] = False
+    near(out[mine.to(device)], want[mine], tol[mine])
+    assert bool((out[~mine.to(device)] == 7.0).all())
+
+
+@gpu
+def test_captured_prompts_replayed_with_other_lengths():
+    """Prompt rows with sums in a graph; lengths, rows and row bounds change between replays."""
+    device, heads, kv, D = "cuda:0", 8, 2, 64
+    plans = [([900, 400, 30], [20, 7, 30]), ([1000, 33, 64], [1, 33, 23]), ([57, 640, 1], [57, 0, 0])]
+    cache, table = filled([1000, 640, 64], 16, kv, D, D, seed=5, device=device)
+    T = 57
+    q, cu, ctx = torch.zeros(T, heads, D, dtype=torch.bfloat16, device=device), i32([0, 0, 0, 0], device), i32([0, 0, 0], device)
+    w, tab = torch.zeros(3, kv, 1000, device=device), i32(table, device)
+
+    def body():
+        return ops.kv8_attention(q, cache, tab, ctx, cu, T, 0.125, weights=w, observe=9, window=500)
+    body()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = body()
+    for j, (lens, new) in enumerate(plans):
+        rows = randn(T, heads, D, seed=50 + j).bfloat16()
+        q.copy_(rows)
+        cu.copy_(i32(cum(new)))
+        ctx.copy_(i32(lens))
+        w.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        want, tol, weight, off = attend(rows[:sum(new)], cache, table, lens, new, 0.125, window=500)
+        near(out[:sum(new)], want, tol)
+        for i, (n, m) in enumerate(zip(lens, new)):
+            last = torch.arange(weight[i].shape[2]) % max(m, 1) >= m - 9
+            assert bool(((w[i, :, :n].cpu().double() - weight[i][:, :, last].sum(2)).abs() <= off[i][:, :, last].sum(2) + 2.0 ** -23 * weight[i].sum(2)).all())
+    assert status(device) == 0
