@@ -4,7 +4,7 @@ A value is its code times the scale of its block and head. Scales are powers of 
 lies in [2^e, 2^(e+1)) and at least 2^-60 (0: nothing but zeros). e4m3 is a floating format, so a power of two costs no precision,
 a block whose scale grows keeps its older codes bit for bit down to its smallest normal value, and codes move between blocks
 exactly. NaN is stored as NaN; infinities count as the largest finite bf16 value. Attention takes blocks whose value scales lie up to
-2^100 apart in one row (those of zeros count as 2^-60).
+2^100 apart in one row (those of zeros count as 2^-80).
 
 Sequences are given as everywhere in ``ops``: ``block_table`` int32 [sequences, blocks], ``ctx_lens`` int32 the tokens a sequence
 holds with the call's rows, ``cu_q`` int32 [sequences + 1] bounds of its rows, which are the last of its tokens. On CUDA every

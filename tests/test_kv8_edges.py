@@ -368,3 +368,46 @@ def test_captured_prompts_replayed_with_other_lengths():
             last = torch.arange(weight[i].shape[2]) % max(m, 1) >= m - 9
             assert bool(((w[i, :, :n].cpu().double() - weight[i][:, :, last].sum(2)).abs() <= off[i][:, :, last].sum(2) + 2.0 ** -23 * weight[i].sum(2)).all())
     assert status(device) == 0
+
+
+@gpu
+def test_blocks_behind_4_gigabytes():
+    """Offsets that pass 32 bits: everything in the last blocks of a cache of 4.6 GB of keys and as much of values, bit for bit as in a
+    small one."""
+    device, page, kv, heads, D, lens = "cuda:0", 64, 4, 8, 256, [300, 70]
+    results = []
+    for blocks in (30, 70000):
+        cache = ops.Kv8Cache.empty(blocks, page, kv, D, device=device)
+        top = blocks - 1
+        table = i32([[top - 2 * j - i for j in range(5)] for i in range(2)], device)
+        dst = i32([[top - 10 - 2 * j - i for j in range(2)] for i in range(2)], device)
+        x = randn(sum(lens), kv, D, seed=1).bfloat16().to(device)
+        ops.kv8_append(cache, x, x, table, i32(lens, device), i32(cum(lens), device), 300)
+        got = []
+        for new in ([1, 1], [40, 3]):
+            q = randn(sum(new), heads, D, seed=2).bfloat16().to(device)
+            w = torch.zeros(2, kv, 300, device=device)
+            got += [ops.kv8_attention(q, cache, table, i32(lens, device), i32(cum(new), device), max(new), 0.06, weights=w), w]
+        got += list(ops.kv8_evict(cache, table, i32(lens, device), w, 100, dst, 2, 30))
+        ids = torch.cat([table.flatten(), dst.flatten()]).long()
+        got += [t[ids] for t in (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)]
+        results.append(got)
+        del cache
+    assert status(device) == 0 and bool(results[0][0].float().abs().amax() > 0)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("new", [1, 40])
+def test_zero_values_that_take_nearly_all_of_the_weight(device, new):
+    """Keys with zero values 44 above the others in score: what is left of the others' weight, 2^-60, keeps its bits."""
+    n, heads, D = 200, 8, 16
+    k, v = randn(n, 1, D, seed=1) * 0.1, randn(n, 1, D, seed=2) * 2.0 ** -10
+    k[32:48], v[32:48] = 5.5, 0
+    cache, table = holding(k, v, 16, device)
+    q = torch.ones(new, heads, D, dtype=torch.bfloat16)
+    want, tol, _, _ = attend(q, cache, table, [n], [new], 0.5)
+    assert 2.0 ** -90 < float(want.abs().max()) < 2.0 ** -60
+    near(call(device, q, cache, table, [n], [new], 0.5), want, tol)
+    assert status(device) == 0
