@@ -25,7 +25,7 @@
 // many stages as fit (six of 32 KB for heads of 128), and the tiles' scales. Warp 10: the next piece's queries. Warp 11: P V. Code
 // that runs once a piece or rarely is kept short: unrolled over the heads it was fetched at 6000 clocks a piece.
 //
-// 16 sequences of 8192 tokens, 32 / 4 heads of 128: 37.6 us = 3.6 TB/s with the join, 0.55 of the measured copy rate. In its steady
+// 16 sequences of 8192 tokens, 32 / 4 heads of 128: 38.2 us = 3.5 TB/s with the join, 0.54 of the measured copy rate. In its steady
 // state a tile takes an SM 1200 to 1370 clocks, which is the memory's rate; the rest is the launch's beginning (lengths, table,
 // first keys: dependent reads, and instructions fetched behind them) and its end.
 #include "kv8_dev.cuh"

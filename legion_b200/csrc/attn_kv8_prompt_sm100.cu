@@ -11,7 +11,7 @@
 // A key's scale multiplies its score, a value's scale 2^e joins the exponent, z = s + e, and the running reference is taken over
 // z, so P stays in the range of a half; the denominator adds exp(z) 2^-e. Both come per 8 keys from a ring in shared memory.
 //
-// 8192 tokens, 32 / 4 heads of 128: 746 us = 737 TFLOP/s, 0.44 of the measured bf16 rate. A pair of row tiles and 128 keys take 4400
+// 8192 tokens, 32 / 4 heads of 128: 730 us = 753 TFLOP/s, 0.45 of the measured bf16 rate. A pair of row tiles and 128 keys take 4400
 // clocks, tensor cores and exponentials 2050 each: a row tile's softmax, P V and next scores follow one another (two score tiles
 // and two outputs fill tensor memory), and score MMAs run at shared memory's full rate beside the expanded values.
 //

@@ -4,7 +4,7 @@
 // between the search for the largest magnitude and the encoding, so every input byte is read once:
 //     s' = max(s, 2^(floor(log2 amax) - 7)),   code = e4m3(x / s'),   older codes = e4m3(code * s / s')
 // A block whose first cell is written begins anew (s = 0, other cells become zero). Blocks belong to one sequence, so a CTA has
-// its block to itself and nothing depends on the order of CTAs. 8192 tokens, 4 heads of 128: 9.6 us = 2.6 TB/s, where lengths,
+// its block to itself and nothing depends on the order of CTAs. 8192 tokens, 4 heads of 128: 9.7 us = 2.6 TB/s, where lengths,
 // table and rows are dependent reads; a token for each of 16 sequences is bound by its launch.
 #include "kv8_dev.cuh"
 

@@ -45,8 +45,8 @@ __device__ __forceinline__ float kv8_scale_of(float amax) {
 __device__ __forceinline__ float kv8_inverse(float scale) { return scale > 0.f ? __uint_as_float(0x7f000000u - __float_as_uint(scale)) : 0.f; }
 // A value scale joins the exponents of its keys' weights. A scale of 0, nothing but zeros, counts as 2^-80: its keys belong to the
 // denominator alone, and with a larger scale they would set the reference that other blocks' weights keep their bits below (with 2^0 a
-// block of zeros cost values of 2^-20 a tenth of their size, with 2^-60 it cost keys of 2^-55 of its weight). Below that their own
-// exponentials would run out of range beside scales above 2^20.
+// block of zeros cost values of 2^-20 a fifth of their size in decode, with 2^-60 a weight of 2^-60 beside it most of its bits). With a
+// smaller one their own exponentials would run out of range beside scales above 2^20.
 __device__ __forceinline__ float kv8_value_scale(float scale) { return scale > 0.f ? scale : 0x1p-80f; }
 __device__ __forceinline__ int kv8_log2(float scale) { return max(-120, min(120, int(__float_as_uint(scale) >> 23) - 127)); }
 
