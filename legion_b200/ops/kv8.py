@@ -11,8 +11,8 @@ holds with the call's rows, ``cu_q`` int32 [sequences + 1] bounds of its rows, w
 call enqueues on the current stream, takes its scratch from the allocator (calls on other streams and captured graphs share none)
 and checks shapes, types and devices; what is wrong with them raises ValueError. What lies in tensors is checked by the kernels, which
 record it in the workspace's status word: table entries outside the cache are not followed, attention leaves out a sequence whose rows or
-length do not fit the call, its table or its sums, eviction takes a length only as far as these reach. CPU tensors run the float32 forms
-of ``ops.reference``, where such a length raises ValueError.
+length do not fit the call or its table and adds nothing to sums that are shorter than the length, eviction takes a length only as far as
+table and sums reach. CPU tensors run the float32 forms of ``ops.reference``, where such a length raises ValueError.
 """
 from __future__ import annotations
 

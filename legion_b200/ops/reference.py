@@ -736,7 +736,7 @@ def kv8_evict(cache, block_table, ctx_lens, weights, budget: int, dst_table, kee
     kept = torch.full((B, kv, budget), -1, dtype=torch.int32, device=weights.device)
     sums = torch.zeros(B, kv, budget, device=weights.device)
     for i in range(B):
-        n = int(ctx_lens[i])
+        n = max(0, int(ctx_lens[i]))
         for h in range(kv):
             w = weights[i, h, :n]
             if n <= budget:

@@ -411,3 +411,19 @@ def test_zero_values_that_take_nearly_all_of_the_weight(device, new):
     assert 2.0 ** -90 < float(want.abs().max()) < 2.0 ** -60
     near(call(device, q, cache, table, [n], [new], 0.5), want, tol)
     assert status(device) == 0
+
+
+@pytest.mark.parametrize("device", WHERE)
+def test_lengths_below_zero_hold_nothing(device):
+    cache, table = filled([20, 20], 16, 2, 32, 32, device=device)
+    before, lens, x = on(cache, "cpu"), i32([-3, 20], device), randn(2, 2, 32).bfloat16().to(device)
+    tab, cu = i32(table, device), i32([0, 1, 1], device)
+    ops.kv8_append(cache, x, x, tab, lens, cu, 1)
+    w = torch.rand(2, 2, 20, generator=gen(1)).to(device)
+    kept = ops.kv8_evict(cache, tab, lens, w, 8, i32([[5], [6]], device))
+    assert kept[0].tolist() == [0, 8] and bool((kept[1][0] == -1).all()) and not bool(kept[2][0].any())
+    sums = w.clone()
+    assert not bool(ops.kv8_attention(x[:1].repeat(1, 2, 1), cache, tab[:1], lens[:1], cu[:2], 1, 0.2, weights=w[:1]).any())
+    assert torch.equal(w, sums) and status(device) == 0
+    for n in cache.__slots__:
+        assert torch.equal(getattr(before, n)[:6].view(torch.uint8), getattr(cache, n)[:6].cpu().view(torch.uint8))
