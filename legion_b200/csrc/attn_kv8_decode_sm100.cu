@@ -629,12 +629,9 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         float f1 = m1 == -INFINITY ? (l1 == l1 ? 0.f : 1.f) : ex2(m1 - m);
         float den = l0 * f0 + l1 * f1, top = m == -INFINITY ? m : m - OFFSET;
         if (q < gn && whole) {
-          if (p.a.sink) {
-            const float sk = p.a.sink[head0 + q] * 1.4426950408889634f;
-            if (top == -INFINITY && den == 0.f) { top = sk; den = 1.f; }
-            else den += ex2(sk - top);
-          }
-          const float inv = den > 0.f || den != den ? 1.f / den : 0.f;
+          float f = 1.f;
+          if (p.a.sink) f = kv8_add_sink(p.a.sink[head0 + q] * 1.4426950408889634f, top, den);
+          const float inv = den > 0.f || den != den ? f / den : 0.f;
           f0 *= inv;
           f1 *= inv;
           if (p.a.lse) p.a.lse[long(row) * p.a.Hq + head0 + q] = den > 0.f ? top + log2f(den) : -INFINITY;

@@ -597,11 +597,11 @@ kv8_prompt_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
       } else {
         if (p.a.sink) {
-          const float sk = (row_ok ? p.a.sink[head] : 0.f) * 1.4426950408889634f;
-          if (top == -INFINITY && den == 0.f) { top = sk; den = 1.f; }
-          else den += ex2(sk - top);
+          const float f = kv8_add_sink((row_ok ? p.a.sink[head] : 0.f) * 1.4426950408889634f, top, den);
+          inv = den > 0.f || den != den ? f / den : 0.f;
+        } else {
+          inv = den > 0.f || den != den ? 1.f / den : 0.f;
         }
-        inv = den > 0.f || den != den ? 1.f / den : 0.f;
         if (p.a.lse && row_ok) p.a.lse[t * p.a.Hq + head] = den > 0.f ? top + log2f(den) : -INFINITY;
       }
 #pragma unroll 1

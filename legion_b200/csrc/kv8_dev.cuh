@@ -56,6 +56,20 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+// A sink (log2) joins a denominator of exponentials relative to 2^top, both then relative to the larger: what the factor returned leaves
+// of sums so far. (Relative to `top` alone a sink 2^40 above keys of zero values would be infinite.)
+__device__ __forceinline__ float kv8_add_sink(float sk, float& top, float& den) {
+  if (top == -INFINITY && den == 0.f) {
+    top = sk;
+    den = 1.f;
+    return 0.f;
+  }
+  const float m = fmaxf(top, sk), f = ex2(top - m);
+  den = den * f + ex2(sk - m);
+  top = m;
+  return f;
+}
+
 // A kernel's shared memory limit is a setting per device: set at its first launch on each.
 struct DeviceOnce {
   std::atomic<uint64_t> done{0};

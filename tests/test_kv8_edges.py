@@ -427,3 +427,22 @@ def test_lengths_below_zero_hold_nothing(device):
     assert torch.equal(w, sums) and status(device) == 0
     for n in cache.__slots__:
         assert torch.equal(getattr(before, n)[:6].view(torch.uint8), getattr(cache, n)[:6].cpu().view(torch.uint8))
+
+
+@pytest.mark.parametrize("device", WHERE)
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("n", [100, 1000])
+def test_a_sink_that_takes_nearly_all_of_the_weight(device, new, n):
+    """A sink 44 above every score, values of zero beside others: keys keep their 2^-60 of a weight."""
+    heads, D = 8, 16
+    k, v = torch.full((n, 1, D), -5.5), randn(n, 1, D, seed=2)
+    v[32:48] = 0
+    cache, table = holding(k, v, 16, device)
+    q, sink = torch.ones(new, heads, D, dtype=torch.bfloat16), torch.zeros(heads)
+    for lens, window in (([n], 0), ([n], 45), ([47], 5), ([47], 0)):      # (the last rows of 47 see zero values alone through a window of 5)
+        want, tol, weight, off = attend(q, cache, table, lens, [new], 0.5, window=window, sink=sink)
+        sums = torch.zeros(1, 1, n, device=device)
+        near(call(device, q, cache, table, lens, [new], 0.5, window=window, sink=sink, weights=sums), want, tol)
+        got, full, err = sums[0, 0, :lens[0]].cpu().double(), weight[0][0].sum(1), off[0][0].sum(1)
+        assert float(full.max()) < 2.0 ** -50 and bool(((got - full).abs() <= err + 2.0 ** -23 * full).all())
+    assert status(device) == 0
