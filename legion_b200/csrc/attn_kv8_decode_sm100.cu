@@ -25,7 +25,7 @@
 // many stages as fit (six of 32 KB for heads of 128), and the tiles' scales. Warp 10: the next piece's queries. Warp 11: P V. Code
 // that runs once a piece or rarely is kept short: unrolled over the heads it was fetched at 6000 clocks a piece.
 //
-// 16 sequences of 8192 tokens, 32 / 4 heads of 128: 38.2 us = 3.5 TB/s with the join, 0.54 of the measured copy rate. In its steady
+// 16 sequences of 8192 tokens, 32 / 4 heads of 128: 37.4 us = 3.6 TB/s with the join, 0.55 of the measured copy rate. In its steady
 // state a tile takes an SM 1200 to 1370 clocks, which is the memory's rate; the rest is the launch's beginning (lengths, table,
 // first keys: dependent reads, and instructions fetched behind them) and its end.
 #include "kv8_dev.cuh"
@@ -38,6 +38,7 @@ struct DecodeArgs {
   Kv8Cache c;
   Kv8Seqs s;
   Kv8Attn a;
+  int cells;                    // of a row of the table
   float scale_log2, cap_k;      // as in softcap_r: soft-capped scores have 2 cap log2(e) in scale_log2
   float* part;                  // [CTAs][2][NQ][dv + 2]: sums over the values, reference (log2), denominator; 0: the piece that a
                                 // CTA begins with, 1: the one it ends with, where they are parts of a group
@@ -183,7 +184,7 @@ kv8_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   auto read_seq = [&](int b) -> int2 {
     const int row = p.s.cu[b], end = p.s.cu[b + 1];
     const int ctx = max(p.s.ctx[b], 0);
-    const bool good = row >= 0 && end <= p.s.T && end <= row + 1 && (end <= row || ctx <= long(p.s.width) * c.page);
+    const bool good = row >= 0 && end <= p.s.T && end <= row + 1 && (end <= row || ctx <= p.cells);
     if (!good && blockIdx.x == 0) atomicCAS(p.s.status, 0, ST_BAD_ARGS);
     return make_int2(ctx, good && end == row + 1 ? row : -1);
   };
@@ -793,7 +794,7 @@ int kv8_decode_launch(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& a, int
     kv8_set_error(tmap_last_error());
     return 1;
   }
-  DecodeArgs p{c, s, a, a.scale * 1.4426950408889634f, 0.f, part, reinterpret_cast<int4*>(meta)};
+  DecodeArgs p{c, s, a, s.width * c.page, a.scale * 1.4426950408889634f, 0.f, part, reinterpret_cast<int4*>(meta)};
   const bool cap = a.softcap > 0.f;
   if (cap) {
     p.cap_k = 2.f * 1.4426950408889634f * a.scale / a.softcap;
